@@ -235,6 +235,101 @@ int wx_stream_spin(void* stream, int32_t microseconds);
 int wx_stream_create_exclusive(int32_t device, void** out_stream);
 int wx_stream_destroy(void* stream);
 
+/* ---- paged key/value cache and drafted decoding -----------------------------------------------------------------------------
+ * NO COUNTERPART IN THE REFERENCE (its decoder keeps one dense cache per call).  For decoding that checks several drafted tokens
+ * of every sequence in one pass (wx_draft_step runs the engine's own decoder this way) and for programs that keep their own paged
+ * cache.  A cache is a description of buffers that the CALLER owns; nothing is allocated, no call waits for the GPU, and every call
+ * may be captured into a graph.  A cache belongs to one stream of work at a time: calls on one cache must not overlap, and neither
+ * may replays of graphs captured from them.
+ *
+ * A sequence slot s holds d_held[s] pages, d_table[s][0 .. held), and d_lens[s] committed tokens; token t lies in row t % page_size of
+ * page d_table[s][t / page_size], in every layer.  d_refs[p] counts the slots that hold page p; a page with 0 is free.  An empty
+ * cache: table -1, refs, lens and held 0.  Rows behind the committed ones are scratch (the rows of drafted tokens).
+ *
+ * Lists of slots (d_seqs, d_dst) are device arrays of n <= max_seqs ids.  d_status (may be NULL) receives a wx_status for each entry:
+ * WX_ERR_INVALID where the id is out of range, appears earlier in the list or asks for what the call does not allow, WX_ERR_NOMEM
+ * where free pages or table columns ran out; such an entry changes nothing.  n == 0 is allowed and does nothing. */
+typedef struct {
+    void *d_k, *d_v;                   /* pools [n_layer][n_pages][n_kv_head][page_size][head_dim], 16-byte aligned */
+    int32_t* d_table;                  /* [max_seqs][max_pages] */
+    int32_t* d_refs;                   /* [n_pages], 16-byte aligned */
+    int32_t* d_lens;                   /* [max_seqs] */
+    int32_t* d_held;                   /* [max_seqs] */
+    int32_t* d_work;                   /* wx_cache_work_ints() ints, 16-byte aligned; contents are never kept between calls */
+    int32_t n_layer, n_pages, n_kv_head, page_size, head_dim;   /* page_size: 16, 32, 64, 128 or 256; head_dim: 64 or 128 */
+    int32_t max_seqs, max_pages;       /* max_seqs <= 8192 */
+    int32_t precision;                 /* WX_PREC_F32 or WX_PREC_BF16 */
+    int32_t device;                    /* HIP device ordinal of all buffers */
+} wx_cache;
+int64_t wx_cache_work_ints(const wx_cache* c);
+/* slot d_seqs[i] keeps its first d_lens[i] tokens (0 <= d_lens[i] <= its length; d_lens NULL: none, the slot is freed); pages behind
+ * the last kept token are given up */
+int wx_cache_truncate(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_lens, int32_t n, int32_t* d_status, void* stream);
+/* slot d_dst[i] becomes what slot d_src[i] was before the call: its committed tokens, on the same pages.  What d_dst[i] held is given
+ * up.  A source may appear any number of times, and as a destination too (the beams of a window, reordered in place). */
+int wx_cache_fork(const wx_cache* c, const int32_t* d_dst, const int32_t* d_src, int32_t n, int32_t* d_status, void* stream);
+/* room for d_extra[i] (d_extra NULL: `extra`) more tokens behind the committed ones, in pages that no other slot holds.  Pages are
+ * taken lowest number first, in the order of the list; an entry that does not fit the free pages, and every later one that needs
+ * a page, changes nothing (WX_ERR_NOMEM).  A partly filled last page that another slot holds too is replaced by a copy of its
+ * committed rows. */
+int wx_cache_reserve(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_extra, int32_t extra, int32_t n, int32_t* d_status,
+                     void* stream);
+/* rows 0 .. d_counts[i]-1 (NULL: n_nodes) of slot d_seqs[i] to the places behind its committed tokens, in layers layer0 ..
+ * layer0 + n_layers - 1; the length stays.  Element (l, i, j, h, x) of the rows lies at [l*layer_stride + i*seq_stride + j*node_stride
+ * + h*head_stride + x] (strides in elements, multiples of 16 bytes).  Entries whose places are not reserved are left out. */
+int wx_cache_append(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_counts, int32_t n, int32_t n_nodes, int32_t layer0,
+                    int32_t n_layers, const void* d_k, const int64_t* k_strides /* layer, seq, node, head */, const void* d_v,
+                    const int64_t* v_strides, void* stream);
+/* the accepted path of a draft: the row at length + d_path[i][k] moves to length + k for k < d_counts[i], in every layer, and the
+ * length grows by d_counts[i].  d_path [n][n_nodes] strictly ascending from >= 0 within the reserved rows. */
+int wx_cache_commit(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_path, const int32_t* d_counts, int32_t n, int32_t n_nodes,
+                    int32_t* d_status, void* stream);
+/* the live pages move together: with L live pages, the i-th live page numbered L or more moves to the i-th free page below L, and the
+ * tables of all slots follow.  *d_n_live = L; pages L and up are free afterwards. */
+int wx_cache_compact(const wx_cache* c, int32_t* d_n_live, void* stream);
+
+/* attention of n_nodes <= 64 drafted tokens of each of n sequences over layer `layer` of a cache: node i of a sequence attends the
+ * committed tokens, itself and its ancestors.  d_parents [n][n_nodes]: the parent of node i, < i, or -1 where it follows the
+ * committed tokens directly (NULL: a chain).  d_counts[i] (NULL: n_nodes) nodes are there; the rows of the others, and of a sequence
+ * id -1 (padding of a batch), come out as 0.  With d_kn / d_vn the nodes' keys and values are appended behind the committed tokens by the same
+ * call (as wx_cache_append does; the ids must be distinct then), without (both NULL) they lie there.  A sequence id out of range, rows that are not reserved, a
+ * second entry of the same id in an appending call, or a parent out of range (and its descendants) give rows of NaN and append
+ * nothing.  n_nodes == 1 is the ordinary decode step.  n_head: query heads, a multiple of n_kv_head up to 16 x as many; head h reads key/value head
+ * h / (n_head / n_kv_head).  Strides in elements: heads' rows are contiguous and 16-byte aligned.  Softmax and sums in fp32; bf16
+ * caches round the probabilities to bf16 for the product with the values.  What masked rows hold (NaN, infinities) has no effect.
+ * split_tokens: the committed tokens are cut into pieces that workgroups take side by side; 0 = by the size of the batch; > 0 = pieces
+ * of that many tokens (rounded up to a multiple of 64), so that a sequence's result does not depend on what else is in the batch. */
+typedef struct {
+    int32_t layer, n, n_nodes, n_head;
+    const int32_t *d_seqs, *d_parents, *d_counts;
+    const void* d_q; int64_t q_seq, q_node, q_head;
+    const void* d_kn; int64_t kn_seq, kn_node, kn_head;
+    const void* d_vn; int64_t vn_seq, vn_node, vn_head;
+    void* d_out; int64_t o_seq, o_node, o_head;
+    float scale;
+    int32_t split_tokens;
+    void* d_work; int64_t work_bytes;  /* wx_tree_attention_work_bytes(), 16-byte aligned; contents are never kept */
+} wx_tree_attn;
+int64_t wx_tree_attention_work_bytes(const wx_cache* c, const wx_tree_attn* a);
+int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream);
+
+/* greedy verification of a draft: for every node the id with the largest logit (the lowest id of equals) among those that d_suppress
+ * (one byte per id, NULL: none) does not mask, and its log-probability among them; then, from node 0 on, the path of nodes each of
+ * which is the first child of the one before whose token is that one's id.  d_next is the id picked at the path's end.  NaN logits
+ * count as masked; a node with nothing left has id -1 and log-probability -inf.  Nodes that d_counts leaves out: id -1, 0. */
+typedef struct {
+    int32_t n, n_nodes, n_vocab, precision;                /* n_nodes <= 64; precision of the logits */
+    int32_t device;
+    const void* d_logits; int64_t l_seq, l_node;           /* element strides, rows contiguous */
+    const int32_t *d_tokens, *d_parents, *d_counts;        /* [n][n_nodes], as wx_tree_attn */
+    const uint8_t* d_suppress;                             /* [n_vocab] or NULL */
+    int32_t* d_pick; float* d_logprob; int32_t* d_path;    /* [n][n_nodes]; the path is padded with -1 */
+    int32_t *d_n_accept, *d_next;                          /* [n] */
+    void* d_work; int64_t work_bytes;                      /* wx_tree_verify_work_bytes() */
+} wx_tree_check;
+int64_t wx_tree_verify_work_bytes(const wx_tree_check* a);
+int wx_tree_verify(const wx_tree_check* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,28 @@ class WxDecodeOpts(ctypes.Structure):
         "max_initial_timestamp_index", "use_graph", "check_interval", "profile_stride")]
 
 
+class WxCache(ctypes.Structure):
+    _fields_ = [(n, c_vp) for n in ("d_k", "d_v", "d_table", "d_refs", "d_lens", "d_held", "d_work")] + [(n, c_i32) for n in (
+        "n_layer", "n_pages", "n_kv_head", "page_size", "head_dim", "max_seqs", "max_pages", "precision", "device")]
+
+
+class WxTreeAttn(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("layer", "n", "n_nodes", "n_head")] + [
+        ("d_seqs", c_vp), ("d_parents", c_vp), ("d_counts", c_vp),
+        ("d_q", c_vp), ("q_seq", c_i64), ("q_node", c_i64), ("q_head", c_i64),
+        ("d_kn", c_vp), ("kn_seq", c_i64), ("kn_node", c_i64), ("kn_head", c_i64),
+        ("d_vn", c_vp), ("vn_seq", c_i64), ("vn_node", c_i64), ("vn_head", c_i64),
+        ("d_out", c_vp), ("o_seq", c_i64), ("o_node", c_i64), ("o_head", c_i64),
+        ("scale", ctypes.c_float), ("split_tokens", c_i32), ("d_work", c_vp), ("work_bytes", c_i64)]
+
+
+class WxTreeCheck(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("n", "n_nodes", "n_vocab", "precision", "device")] + [
+        ("d_logits", c_vp), ("l_seq", c_i64), ("l_node", c_i64), ("d_tokens", c_vp), ("d_parents", c_vp), ("d_counts", c_vp),
+        ("d_suppress", c_vp), ("d_pick", c_vp), ("d_logprob", c_vp), ("d_path", c_vp), ("d_n_accept", c_vp), ("d_next", c_vp),
+        ("d_work", c_vp), ("work_bytes", c_i64)]
+
+
 # name -> (restype, argtypes); exactly the declarations of include/whisper_amd.h
 PROTOTYPES = {
     "wx_last_error": (ctypes.c_char_p, []),
@@ -61,6 +83,17 @@ PROTOTYPES = {
     "wx_stream_spin": (c_i32, [c_vp, c_i32]),
     "wx_stream_create_exclusive": (c_i32, [c_i32, ctypes.POINTER(c_vp)]),
     "wx_stream_destroy": (c_i32, [c_vp]),
+    "wx_cache_work_ints": (c_i64, [c_vp]),
+    "wx_cache_truncate": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "wx_cache_fork": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "wx_cache_reserve": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
+    "wx_cache_append": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "wx_cache_commit": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
+    "wx_cache_compact": (c_i32, [c_vp, c_vp, c_vp]),
+    "wx_tree_attention_work_bytes": (c_i64, [c_vp, c_vp]),
+    "wx_tree_attention": (c_i32, [c_vp, c_vp, c_vp]),
+    "wx_tree_verify_work_bytes": (c_i64, [c_vp]),
+    "wx_tree_verify": (c_i32, [c_vp, c_vp]),
 }
 
 _lib = None

@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "csrc", "build")
 LIB = os.path.join(HERE, "libwhisper_amd.so")
-SOURCES = ["mel.hip", "gemm.hip", "attention.hip", "flash.hip", "xattn.hip", "elementwise.hip", "beam.hip", "engine.hip"]
+SOURCES = ["mel.hip", "gemm.hip", "attention.hip", "flash.hip", "xattn.hip", "elementwise.hip", "beam.hip", "pages.hip", "tree.hip", "engine.hip"]
 # packed fp32 instructions are switched off: some of their forms have given wrong results on MI355X, without an error.  (The host
 # pass warns that it does not know the feature.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",

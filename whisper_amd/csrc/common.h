@@ -3,8 +3,11 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include "../../include/whisper_amd.h"
 
 namespace wx {
+
+int set_error(int code, const char* msg);      // records wx_last_error()'s message and returns the code (engine.hip)
 
 typedef __bf16 bf16;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -292,5 +295,18 @@ struct BeamArgs {
     int without_timestamps = 1, suppress_blank = 1, max_initial_ts = 50;
 };
 int launch_beam_step(const BeamArgs& s, hipStream_t st);   // topk -> select -> gather -> commit (position += 1)
+
+// ---- paged cache (pages.hip) and tree attention / verification (tree.hip) ----------------------------------
+// Every call runs with its buffers' device current and restores the caller's on the way out.
+struct OnDevice {
+    int prev = -1, dev;
+    explicit OnDevice(int d) : dev(d) {
+        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (prev != dev) (void)hipSetDevice(dev);
+    }
+    ~OnDevice() { if (prev >= 0 && prev != dev) (void)hipSetDevice(prev); }
+};
+// nullptr, or what is wrong with a cache's description (host-side check of every call)
+const char* cache_fault(const wx_cache* c);
 
 }  // namespace wx

@@ -17,6 +17,7 @@ using namespace wx;
 
 static thread_local std::string g_err;
 static int fail(int code, const std::string& msg) { g_err = msg; return code; }
+namespace wx { int set_error(int code, const char* msg) { return fail(code, msg); } }
 
 #define HIP_TRY(expr)                                                                                   \
     do {                                                                                                \
