@@ -10,29 +10,113 @@ namespace wx {
 constexpr int TR_NODES = 64;              // nodes a sequence: one bit each of a mask
 constexpr float TR_LOG2E = 1.4426950408889634f;
 
-// What an entry of the call is: 0 = its rows are 0 (padding), 1 = attend, 2 = refused (NaN).  Every thread of the workgroup; the same
-// answer in every workgroup and in the append launch (cache_append_kernel).
-__device__ __forceinline__ int tree_entry(const wx_cache& c, const wx_tree_attn& a, int i, int* len, int* count) {
+// How the committed tokens of a batch are cut into pieces that workgroups take side by side.  A sequence has ceil(len / KT) tiles of
+// committed tokens and `tree_tiles` behind them; a piece is at most `per` tiles.  per == 0: by the batch, so that about `target`
+// pieces come out (one round of workgroups over the chip), but not below `least` tiles, which keeps a merge worth its traffic.
+struct TreePlan {
+    int row_blocks;          // workgroups over the rows (nodes x query heads of a key / value head)
+    int tree_tiles, per, least, target;
+    int single;              // 1: no sequence that the tables can hold has a second piece
+    int shift;               // log2 of the page size
+    int slots;               // pieces x sequences that the grid has room for
+    int rows;                // rows a workgroup
+    float* part;             // [slots][n_kv_head][row_blocks][rows][D + 2]: output, maximum and sum of a piece (more than one piece only)
+};
+
+__device__ __forceinline__ int tree_tiles_of(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, int i, int kt) {
     const int s = a.d_seqs[i];
-    *len = 0;
-    *count = a.d_counts ? min(max(a.d_counts[i], 0), a.n_nodes) : a.n_nodes;
-    if (s == -1) return 0;
-    int bad = s < 0 || s >= c.max_seqs;
-    if (!bad) {
-        const int l = c.d_lens[s], held = min(c.d_held[s], c.max_pages);
-        *len = l;
-        bad = l < 0 || (int64_t)l + *count > (int64_t)held * c.page_size;
-        if (!bad) {
-            const int32_t* row = c.d_table + (int64_t)s * c.max_pages;
-            const int first_own = a.d_kn ? l / c.page_size : 0x7fffffff;
-            for (int p = threadIdx.x; p * c.page_size < l + *count; p += blockDim.x) {
-                const int page = row[p];
-                if ((unsigned)page >= (unsigned)c.n_pages || (p >= first_own && c.d_refs[page] != 1)) bad = 1;
-            }
-        }
-        if (a.d_kn) for (int j = threadIdx.x; j < i; j += blockDim.x) bad |= a.d_seqs[j] == s;
+    const int len = s >= 0 && s < c.max_seqs ? min(max(c.d_lens[s], 0), c.max_pages << p.shift) : 0;
+    return (len + kt - 1) / kt + p.tree_tiles;
+}
+// one wave: the sequence and piece that slot g stands for, how many pieces the sequence has and its first slot; false: none
+__device__ __forceinline__ bool tree_locate(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, int kt, int g, int lane, int* seq, int* piece, int* pieces) {
+    if (p.single) { *seq = g; *piece = 0; *pieces = 1; return g < a.n; }
+    int per = p.per;
+    if (per == 0) {
+        int64_t all = 0;
+        for (int i = lane; i < a.n; i += 64) all += tree_tiles_of(c, a, p, i, kt);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
+        const int64_t units = (int64_t)c.n_kv_head * p.row_blocks;
+        per = (int)max((int64_t)p.least, (all * units + p.target - 1) / p.target);
     }
-    return __syncthreads_or(bad) ? 2 : 1;
+    int first = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 64) {
+        const int i = i0 + lane;
+        const int mine = i < a.n ? (tree_tiles_of(c, a, p, i, kt) + per - 1) / per : 0;
+        int upto = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) { const int u = __shfl_up(upto, off); if (lane >= off) upto += u; }
+        const uint64_t past = __ballot(first + upto > g);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            *seq = i0 + at;
+            *pieces = __shfl(mine, at);
+            *piece = g - (first + __shfl(upto, at) - *pieces);
+            return true;
+        }
+        first += __shfl(upto, 63);
+    }
+    return false;
+}
+
+// What a workgroup has to do: sequence entry i, key / value head, block of rows, tiles [t0, t1) of the sequence's n_pre + tree_tiles.
+struct TreeJob {
+    int ok;                  // 0: the rows are 0 (padding, no nodes), 1: attend, 2: refused (NaN)
+    int i, kh, rb, slot, piece, pieces, seq, len, count, n_pre, t0, t1, last;
+};
+
+template <int KT>
+__device__ __forceinline__ bool tree_job(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob* sh, TreeJob& j) {
+    // XCD-aware: consecutive workgroups go to different XCDs, so the row blocks that read the same keys are 8 apart, on one L2
+    const int units = c.n_kv_head, lin = blockIdx.x, x = lin % 8, y = lin / 8;
+    const int w = (y / p.row_blocks) * 8 + x;
+    const int tid = threadIdx.x, slot = w / units;
+    if (slot >= p.slots) return false;
+    if (tid < 64) {
+        int seq = 0, piece = 0, pieces = 0;
+        const bool any = tree_locate(c, a, p, KT, slot, tid, &seq, &piece, &pieces);
+        if (tid == 0) {
+            TreeJob t;
+            t.ok = any ? 1 : -1; t.i = seq; t.kh = w % units; t.rb = y % p.row_blocks; t.slot = slot; t.piece = piece; t.pieces = pieces;
+            t.seq = 0; t.len = 0; t.count = 0; t.n_pre = 0; t.t0 = 0; t.t1 = 0; t.last = 0;
+            if (any) {
+                t.seq = a.d_seqs[seq];
+                t.count = a.d_counts ? min(max(a.d_counts[seq], 0), a.n_nodes) : a.n_nodes;
+                if (t.seq == -1) t.ok = 0;
+                else if (t.seq < 0 || t.seq >= c.max_seqs) t.ok = 2;
+                else {
+                    t.len = c.d_lens[t.seq];
+                    if (t.len < 0 || (int64_t)t.len + t.count > (int64_t)min(c.d_held[t.seq], c.max_pages) << p.shift) t.ok = 2;
+                    else if (t.count == 0) t.ok = 0;
+                    t.n_pre = (min(max(t.len, 0), c.max_pages << p.shift) + KT - 1) / KT;
+                    const int all = t.n_pre + p.tree_tiles, per = (all + pieces - 1) / pieces;
+                    t.t0 = min(all, piece * per); t.t1 = min(all, t.t0 + per);
+                    if (t.t0 == t.t1) t.t0 = t.t1 = 0;                              // a piece may be left without tiles
+                    t.last = t.t1 == all;
+                }
+            }
+            *sh = t;
+        }
+    }
+    __syncthreads();
+    j = *sh;
+    if (j.ok < 0) return false;
+    int bad = 0;
+    if (j.ok == 1) {
+        // the pages of this piece's tiles (of the draft's rows too, which have to be this slot's alone where they are written)
+        const int32_t* row = c.d_table + (int64_t)j.seq * c.max_pages;
+        const bool tail = j.t1 > j.n_pre;
+        const int upto = tail ? j.len + j.count : min(j.len, j.t1 * KT);
+        const int own = a.d_kn && j.last ? j.len >> p.shift : 0x7fffffff;
+        for (int q = (min(j.t0 * KT, j.len) >> p.shift) + tid; q << p.shift < upto; q += 256) {
+            const int page = row[q];
+            if ((unsigned)page >= (unsigned)c.n_pages || (q >= own && c.d_refs[page] != 1)) bad = 1;
+        }
+        if (a.d_kn) for (int k = tid; k < j.i; k += 256) bad |= a.d_seqs[k] == j.seq;
+    }
+    if (__syncthreads_or(bad)) j.ok = 2;
+    return true;
 }
 
 // bit j of the result, on lane i of a wave: node j is node i or one of its ancestors.  *bad: node i hangs on a parent out of range.
@@ -55,92 +139,677 @@ __device__ __forceinline__ uint64_t tree_mask(const int32_t* parents, int lane, 
     return m;
 }
 
-template <typename T> __device__ __forceinline__ void load_f32(const T* p, float* out);      // 16 bytes
-template <> __device__ __forceinline__ void load_f32<float>(const float* p, float* out) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(p);
+
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((ext_vector_type(8))) short i16x8;
+
+// ---- what differs between the element types -----------------------------------------------------------------------------------
+// Both keep the QUERY ROW on the matrix instruction's column (lane & 15 = r, lane >> 4 = g):
+//   S^T[key][row] = K Q^T    A = 16 keys x 64 bytes of a row (lane (g, r): bytes 16 g of key r), B = the query rows the same way
+//   O^T[d][row] += V^T P^T   B = the S^T accumulator in place (lane (g, r) holds keys 4 g + 0..3 of row r), A = V^T out of LDS
+// so the running maximum, sum and rescale factor of a row sit on the lanes that hold its scores and outputs, and P never moves.
+template <typename T> struct Elem;
+template <> struct Elem<bf16> {
+    typedef bf16x8 Frag;
+    static __device__ __forceinline__ f32x4 qk(Frag k, Frag q, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q, c, 0, 0, 0); }
+    static __device__ __forceinline__ bool odd(Frag v) {                        // holds an infinity or a NaN
+        const i32x4 b = __builtin_bit_cast(i32x4, v);
+        bool o = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = v[j];
-}
-template <> __device__ __forceinline__ void load_f32<bf16>(const bf16* p, float* out) {
-    const bf16x8 v = *reinterpret_cast<const bf16x8*>(p);
+        for (int j = 0; j < 4; ++j) o |= (b[j] & 0x7f800000) == 0x7f800000 || (b[j] & 0x7f80) == 0x7f80;
+        return o;
+    }
+    static constexpr int PAD = 32;                                            // bytes behind a V row in LDS: the transposing reads hit every bank once
+};
+template <> struct Elem<float> {
+    typedef f32x4 Frag;
+    static __device__ __forceinline__ f32x4 qk(Frag k, Frag q, f32x4 c) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = (float)v[j];
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j], q[j], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ bool odd(Frag v) {
+        const i32x4 b = __builtin_bit_cast(i32x4, v);
+        bool o = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o |= (b[j] & 0x7f800000) == 0x7f800000;
+        return o;
+    }
+    static constexpr int PAD = 16;
+};
+template <typename F> __device__ __forceinline__ F finite_only(F v) {
+#pragma unroll
+    for (int j = 0; j < (int)(16 / sizeof(v[0])); ++j) { const float x = (float)v[j]; if (!(fabsf(x) < INFINITY)) v[j] = 0; }
+    return v;
 }
 
-// One workgroup a (node, query head, sequence): every thread takes every 256th token with a running maximum, sum and output of its own.
+// The state of RT x 16 rows on a wave: maximum and (this lane's share of the) sum of every row, output.
+template <int D, int RT> struct RowState {
+    float m[RT], l[RT];
+    f32x4 o[D / 16][RT];
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            m[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) o[d][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // scores -> probabilities (in place); c = |scale| log2 e.  A tile that is masked altogether leaves the state alone.
+    template <int NS> __device__ __forceinline__ void softmax(f32x4 (&s)[NS][RT], float c) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float mt = s[0][t][0];
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mt = fmaxf(mt, s[k][t][j]);
+            mt = fmaxf(mt, __shfl_xor(mt, 16));
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const float mn = fmaxf(m[t], mt), base = mn == -INFINITY ? 0.f : mn * c;
+            const float alpha = __builtin_amdgcn_exp2f(fmaf(m[t], c, -base));       // m = -infinity: 0
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { s[k][t][j] = __builtin_amdgcn_exp2f(fmaf(s[k][t][j], c, -base)); sum += s[k][t][j]; }
+            l[t] = fmaf(l[t], alpha, sum);
+            m[t] = mn;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {                      // rare after the first tiles
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) o[d][t] *= alpha;
+            }
+        }
+    }
+    // o += V^T P^T for NS x 16 keys; vb: their rows in LDS, VROW bytes each
+    template <int NS, int VROW> __device__ __forceinline__ void add(const f32x4 (&p)[NS][RT], const char* vb, int g, int r, bf16) {
+#pragma unroll
+        for (int h = 0; h < NS / 2; ++h) {
+            bf16x8 pf[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { pf[t][j] = (bf16)p[2 * h][t][j]; pf[t][4 + j] = (bf16)p[2 * h + 1][t][j]; }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                // lane (g, r) receives V[32 h + 16 u + 4 g + j][16 d + r], j = 0..3, for u = 0, 1
+                const char* p0 = vb + (32 * h + 4 * g + (r >> 2)) * VROW + (16 * d + 4 * (r & 3)) * 2;
+                const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0));
+                const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 16 * VROW));
+                const bf16x8 vf = __builtin_bit_cast(bf16x8, (i16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int t = 0; t < RT; ++t) o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], o[d][t], 0, 0, 0);
+            }
+        }
+    }
+    template <int NS, int VROW> __device__ __forceinline__ void add(const f32x4 (&p)[NS][RT], const char* vb, int g, int r, float) {
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float* row = reinterpret_cast<const float*>(vb + (16 * k + 4 * g + j) * VROW) + r;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const float v = row[16 * d];
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) o[d][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[k][t][j], o[d][t], 0, 0, 0);
+                }
+            }
+    }
+};
+
+// Rows of a sequence's drafted nodes: given with the call, or in the cache behind the committed tokens.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void tree_attention_kernel(wx_cache c, wx_tree_attn a) {
-    constexpr int E = 16 / sizeof(T);
-    __shared__ float sq[D], red[256], so[4][D];
-    __shared__ uint64_t s_mask;
-    __shared__ int s_bad;
-    const int node = blockIdx.x, h = blockIdx.y, i = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
-    int len, count;
-    int what = tree_entry(c, a, i, &len, &count);
+__device__ __forceinline__ const T* node_row(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off,
+                                             int64_t page_e, bool keys, int node) {
+    if (a.d_kn)
+        return keys ? reinterpret_cast<const T*>(a.d_kn) + j.i * a.kn_seq + node * a.kn_node + j.kh * a.kn_head
+                    : reinterpret_cast<const T*>(a.d_vn) + j.i * a.vn_seq + node * a.vn_node + j.kh * a.vn_head;
+    const int t = j.len + node;
+    return reinterpret_cast<const T*>(keys ? c.d_k : c.d_v) + head_off + table[t >> p.shift] * page_e + (int64_t)(t & (c.page_size - 1)) * D;
+}
+
+// The rare end of a tile of drafted rows whose values hold infinities or NaN: the matrix product ran on 0 in their place (0 x NaN would
+// reach the rows that do not attend them); what they give to the rows that do is added here.
+template <typename T, int D, int RT, int NS>
+__device__ __forceinline__ void add_odd_values(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off,
+                                            int64_t page_e, int node0, const f32x4 (&pr)[NS][RT], const uint64_t (&mask)[RT], RowState<D, RT>& st, int g, int r) {
+    for (int k = 0; k < NS * 16 && node0 + k < j.count; ++k) {
+        const T* row = node_row<T, D>(c, a, p, j, table, head_off, page_e, false, node0 + k);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float x = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < NS; ++kk)
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) if (kk == k / 16 && jj == k % 4) x = pr[kk][t][jj];
+            x = __shfl(x, ((k % 16) / 4) * 16 + r);
+            const bool seen = (mask[t] >> (node0 + k)) & 1;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const float v = (float)row[16 * d + 4 * g + jj];
+                    if (seen && !(fabsf(v) < INFINITY)) st.o[d][t][jj] = fmaf(x, v, st.o[d][t][jj]);
+                }
+        }
+    }
+}
+
+// drafted rows -> the cache (one workgroup a sequence and head does it)
+template <typename T, int D>
+__device__ __forceinline__ void append_nodes(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off, int64_t page_e) {
+    constexpr int E = 16 / sizeof(T), PER = D / E;
+    for (int u = threadIdx.x; u < j.count * PER * 2; u += blockDim.x) {
+        const int x = u % PER, node = (u / PER) % j.count, t = j.len + node;
+        const bool keys = u < j.count * PER;
+        T* to = reinterpret_cast<T*>(keys ? c.d_k : c.d_v) + head_off + table[t >> p.shift] * page_e + (int64_t)(t & (c.page_size - 1)) * D + x * E;
+        *reinterpret_cast<i32x4*>(to) = *reinterpret_cast<const i32x4*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, keys, node) + x * E);
+    }
+}
+
+template <typename T> __device__ __forceinline__ void store4(T* to, f32x4 v);
+template <> __device__ __forceinline__ void store4<float>(float* to, f32x4 v) { *reinterpret_cast<f32x4*>(to) = v; }
+template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
+    bf16x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (bf16)v[j];
+    *reinterpret_cast<bf16x4*>(to) = o;
+}
+
+// ---- few rows: every wave has all rows of the workgroup and takes every fourth tile of keys -----------------------------------------
+// Bound by the stream of keys and values.  A tile is 8 KiB of keys (straight into the matrix instruction's registers) and 8 KiB of
+// values (through the wave's own LDS, for the transposing read); the next tile's 16 loads a lane are issued as soon as the scores of
+// this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
+    typedef typename Elem<T>::Frag Frag;
+    constexpr int E = 16 / sizeof(T), KT = 8192 / (D * (int)sizeof(T)), NS = KT / 16, KS = D / (4 * E), CPR = D / E, NV = KT * CPR / 64;
+    constexpr int VROW = D * (int)sizeof(T) + Elem<T>::PAD, VBYTES = KT * VROW, OROW = 68;
+    constexpr int LDS = 4 * VBYTES > 4 * RT * 16 * OROW * 4 ? 4 * VBYTES : 4 * RT * 16 * OROW * 4;
+    __shared__ __attribute__((aligned(16))) char lds[LDS];
+    __shared__ TreeJob s_job;
+    __shared__ uint64_t s_mask[64];
+    __shared__ int s_wrong[64];
+    __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, r = lane & 15;
+    TreeJob j;
+    if (!tree_job<KT>(c, a, p, &s_job, j)) return;
+    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * RT * 16;
+    if (wid == 0 && j.ok == 1) {
+        bool wrong;
+        const uint64_t m = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
+        s_mask[lane] = m; s_wrong[lane] = wrong;
+    }
+    __syncthreads();
+    const int32_t* table = c.d_table + (int64_t)j.seq * c.max_pages;
+    const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)j.kh * c.page_size * D;
+    RowState<D, RT> st;
+    st.init();
+    if (j.ok == 1) {
+        if (a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
+        Frag qf[RT][KS];
+        uint64_t mask[RT];
+        const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f, cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int row = min(row0 + t * 16 + r, rows - 1), node = row / G;
+            const T* q = reinterpret_cast<const T*>(a.d_q) + j.i * a.q_seq + node * a.q_node + (j.kh * G + row % G) * a.q_head;
+            mask[t] = s_mask[node];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                qf[t][ks] = *reinterpret_cast<const Frag*>(q + (ks * 4 + g) * E);
+                if (sign != 1.f) {
+#pragma unroll
+                    for (int x = 0; x < E; ++x) qf[t][ks][x] = (T)((float)qf[t][ks][x] * sign);
+                }
+            }
+        }
+        const T* Kp = reinterpret_cast<const T*>(c.d_k) + head_off;
+        const T* Vp = reinterpret_cast<const T*>(c.d_v) + head_off;
+        char* vb = lds + wid * VBYTES;
+        Frag kf[NS][KS], vr[NV];
+        // a tile's pages: one for each 16 tokens, on lanes 0 .. NS-1
+        auto load_ids = [&](int t) { return table[min(t * KT + 16 * min(lane, NS - 1), j.len - 1) >> p.shift]; };
+        auto load_pre = [&](int t, int ids) {
+            const int last = j.len - 1 - t * KT;                                  // >= 0
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                const int64_t page = (int64_t)__builtin_amdgcn_readlane(ids, k) * page_e;
+                const int at = min(16 * k + r, last), base = t * KT + at;
+                const T* kr = Kp + page + (int64_t)(base & (c.page_size - 1)) * D;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) kf[k][ks] = *reinterpret_cast<const Frag*>(kr + (ks * 4 + g) * E);
+            }
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                constexpr int RPL = 64 / CPR;                                     // rows a load covers
+                const int row = v * RPL + lane / CPR, at = min(row, last), base = t * KT + at;
+                const int64_t page = (int64_t)__builtin_amdgcn_readlane(ids, v * RPL / 16) * page_e;
+                vr[v] = *reinterpret_cast<const Frag*>(Vp + page + (int64_t)(base & (c.page_size - 1)) * D + (lane % CPR) * E);
+            }
+        };
+        auto load_tree = [&](int node0) {
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                const T* kr = node_row<T, D>(c, a, p, j, table, head_off, page_e, true, min(node0 + 16 * k + r, j.count - 1));
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) kf[k][ks] = *reinterpret_cast<const Frag*>(kr + (ks * 4 + g) * E);
+            }
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                vr[v] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, false, min(node0 + (v * 64 + lane) / CPR, j.count - 1)) + (lane % CPR) * E);
+        };
+        // rows of the tile from `live` on are no tokens: their values count as 0 (their scores are masked)
+        auto stage = [&](int live) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int row = (v * 64 + lane) / CPR;
+                Frag x = vr[v];
+                if (row >= live) x = Frag{};
+                *reinterpret_cast<Frag*>(vb + row * VROW + (lane % CPR) * 16) = x;
+            }
+            __builtin_amdgcn_wave_barrier();
+        };
+        auto scores = [&](f32x4 (&s)[NS][RT]) {
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) x = Elem<T>::qk(kf[k][ks], qf[t][ks], x);
+                    s[k][t] = x;
+                }
+        };
+        const int end = min(j.t1, j.n_pre);
+        int t = j.t0 + wid;
+        if (t < end) {
+            int ids = load_ids(t);
+            load_pre(t, ids);
+            ids = load_ids(min(t + 4, j.n_pre - 1));
+            for (; t < end; t += 4) {
+                f32x4 s[NS][RT];
+                const int live = j.len - t * KT;
+                stage(live);
+                scores(s);
+                if (t + 4 < end) {
+                    load_pre(t + 4, ids);
+                    ids = load_ids(min(t + 8, j.n_pre - 1));
+                }
+                if (live < KT) {
+#pragma unroll
+                    for (int k = 0; k < NS; ++k)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            if (16 * k + 4 * g + x >= live)
+#pragma unroll
+                                for (int q = 0; q < RT; ++q) s[k][q][x] = -INFINITY;
+                }
+                st.template softmax<NS>(s, cc);
+                st.template add<NS, VROW>(s, vb, g, r, T());
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        // the drafted rows' tiles go on in the same rotation of waves
+        for (t = j.t0 + wid; t < j.t1; t += 4) {
+            const int node0 = (t - j.n_pre) * KT;
+            if (t < j.n_pre || node0 >= j.count) continue;
+            f32x4 s[NS][RT];
+            load_tree(node0);
+            bool odd = false;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) odd |= Elem<T>::odd(vr[v]);
+            const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+            if (any_odd)
+#pragma unroll
+                for (int v = 0; v < NV; ++v) vr[v] = finite_only(vr[v]);
+            stage(j.count - node0);
+            scores(s);
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) if (!((mask[q] >> (node0 + 16 * k + 4 * g + x)) & 1)) s[k][q][x] = -INFINITY;
+            st.template softmax<NS>(s, cc);
+            st.template add<NS, VROW>(s, vb, g, r, T());
+            if (any_odd) add_odd_values<T, D, RT, NS>(c, a, p, j, table, head_off, page_e, node0, s, mask, st, g, r);
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    // ---- the four waves' states: factors first, then 64 columns of the outputs at a time ---------------------------------------------
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float l = st.l[t];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (g == 0) { s_m[wid][t * 16 + r] = st.m[t]; s_l[wid][t * 16 + r] = l; }
+    }
+    __syncthreads();
+    const bool whole = j.pieces == 1;
+    float* part = whole ? nullptr : p.part + (((int64_t)j.slot * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (RT * 16) * (D + 2);
+    const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
+    float f[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][t * 16 + r]);
+        f[t] = st.m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[t] - M) * cc);
+    }
+    float* o = reinterpret_cast<float*>(lds);
+    for (int half = 0; half < D / 64; ++half) {
+        if (half) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int hh = 0; hh < D / 64; ++hh)
+                    if (hh == half) *reinterpret_cast<f32x4*>(o + ((wid * RT + t) * 16 + r) * OROW + 16 * d + 4 * g) = st.o[hh * 4 + d][t] * f[t];
+        __syncthreads();
+        for (int u = tid; u < RT * 16 * 16; u += 256) {
+            const int row = u / 16, x = (u % 16) * 4, at = row0 + row;
+            if (at >= rows) continue;
+            f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][row]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float m = s_m[w][row];
+                if (m > -INFINITY || m != m || s_l[w][row] != 0.f) L += s_l[w][row] * (m == M ? 1.f : __builtin_amdgcn_exp2f((m - M) * cc));
+                v += *reinterpret_cast<const f32x4*>(o + (w * RT * 16 + row) * OROW + x);
+            }
+            const int node = at / G;
+            if (j.ok == 2) L = __builtin_nanf("");
+            if (whole) {
+                T* out = reinterpret_cast<T*>(a.d_out) + j.i * a.o_seq + node * a.o_node + (j.kh * G + at % G) * a.o_head + half * 64 + x;
+                if (j.ok == 0 || (j.ok == 1 && node >= j.count)) v = f32x4{0.f, 0.f, 0.f, 0.f};
+                else if (j.ok == 2 || s_wrong[node]) v = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+                else v *= 1.f / L;
+                store4<T>(out, v);
+            } else {
+                float* to = part + (int64_t)row * (D + 2);
+                *reinterpret_cast<f32x2*>(to + half * 64 + x) = f32x2{v[0], v[1]};
+                *reinterpret_cast<f32x2*>(to + half * 64 + x + 2) = f32x2{v[2], v[3]};
+                if (x == 0 && half == 0) { to[D] = M; to[D + 1] = L; }
+            }
+        }
+    }
+}
+
+// ---- many rows (bf16): every wave has rows of its own, the workgroup shares the tiles of keys and values ------------------------------
+// Bound by the matrix pipe and the softmax between its two products.  Tiles of 64 keys are loaded into registers while the tile before
+// is worked on, and go to a double-buffered LDS image (one barrier a tile).
+template <int D, int RT>
+__global__ __launch_bounds__(256, 2) void tree_attention_rows_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
+    typedef bf16 T;
+    typedef bf16x8 Frag;
+    constexpr int KT = 64, NS = 4, KS = D / 32, CPR = D / 8, NL = KT * CPR / 256;
+    constexpr int KROW = D * 2, VROW = D * 2 + 32, KBYTES = KT * KROW, VBYTES = KT * VROW;
+    __shared__ __attribute__((aligned(16))) char lds[2 * (KBYTES + VBYTES)];
+    __shared__ TreeJob s_job;
+    __shared__ uint64_t s_mask[64];
+    __shared__ int s_wrong[64];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, r = lane & 15;
+    TreeJob j;
+    if (!tree_job<KT>(c, a, p, &s_job, j)) return;
+    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * 64 * RT + wid * 16 * RT;
+    if (wid == 0 && j.ok == 1) {
+        bool wrong;
+        const uint64_t m = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
+        s_mask[lane] = m; s_wrong[lane] = wrong;
+    }
+    __syncthreads();
+    const int32_t* table = c.d_table + (int64_t)j.seq * c.max_pages;
+    const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)j.kh * c.page_size * D;
+    RowState<D, RT> st;
+    st.init();
+    const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
+    if (j.ok == 1) {
+        if (a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
+        Frag qf[RT][KS];
+        uint64_t mask[RT];
+        const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int row = min(row0 + t * 16 + r, rows - 1), node = row / G;
+            const T* q = reinterpret_cast<const T*>(a.d_q) + j.i * a.q_seq + node * a.q_node + (j.kh * G + row % G) * a.q_head;
+            mask[t] = s_mask[node];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                qf[t][ks] = *reinterpret_cast<const Frag*>(q + (ks * 4 + g) * 8);
+                if (sign != 1.f) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) qf[t][ks][x] = (T)((float)qf[t][ks][x] * sign);
+                }
+            }
+        }
+        const T* Kp = reinterpret_cast<const T*>(c.d_k) + head_off;
+        const T* Vp = reinterpret_cast<const T*>(c.d_v) + head_off;
+        Frag rk[NL], rv[NL];
+        int ids[NL];
+        const int st_row = tid / CPR, st_ch = tid % CPR;                            // load p: row st_row + p * (256 / CPR)
+        constexpr int RPL = 256 / CPR;
+        auto load_ids = [&](int t) {
+#pragma unroll
+            for (int x = 0; x < NL; ++x) ids[x] = table[min(t * KT + st_row + x * RPL, j.len - 1) >> p.shift];
+        };
+        auto load_pre = [&](int t) {
+#pragma unroll
+            for (int x = 0; x < NL; ++x) {
+                const int at = min(t * KT + st_row + x * RPL, j.len - 1);
+                const int64_t off = ids[x] * page_e + (int64_t)(at & (c.page_size - 1)) * D + st_ch * 8;
+                rk[x] = *reinterpret_cast<const Frag*>(Kp + off);
+                rv[x] = *reinterpret_cast<const Frag*>(Vp + off);
+            }
+        };
+        auto load_tree = [&]() {
+#pragma unroll
+            for (int x = 0; x < NL; ++x) {
+                const int node = min(st_row + x * RPL, j.count - 1);
+                rk[x] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, true, node) + st_ch * 8);
+                rv[x] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, false, node) + st_ch * 8);
+            }
+        };
+        // K image: chunk ch of row at slot ch ^ (row & 7): 16 rows' reads of one chunk hit every bank once
+        auto store = [&](int buf, int live) {
+            char* kb = lds + buf * (KBYTES + VBYTES);
+#pragma unroll
+            for (int x = 0; x < NL; ++x) {
+                const int row = st_row + x * RPL;
+                *reinterpret_cast<Frag*>(kb + row * KROW + ((st_ch ^ (row & 7)) << 4)) = rk[x];
+                *reinterpret_cast<Frag*>(kb + KBYTES + row * VROW + (st_ch << 4)) = row < live ? rv[x] : Frag{};
+            }
+        };
+        auto scores = [&](int buf, f32x4 (&s)[NS][RT]) {
+            const char* kb = lds + buf * (KBYTES + VBYTES);
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                const int row = k * 16 + r;
+                Frag kf[KS];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const Frag*>(kb + row * KROW + (((ks * 4 + g) ^ (row & 7)) << 4));
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) x = Elem<T>::qk(kf[ks], qf[t][ks], x);
+                    s[k][t] = x;
+                }
+            }
+        };
+        const int end = min(j.t1, j.n_pre);
+        int buf = 0;
+        if (j.t0 < end) {
+            load_ids(j.t0);
+            load_pre(j.t0);
+            load_ids(min(j.t0 + 1, j.n_pre - 1));
+            store(0, j.len - j.t0 * KT);
+            __syncthreads();
+            for (int t = j.t0; t < end; ++t) {
+                const bool more = t + 1 < end;
+                if (more) { load_pre(t + 1); load_ids(min(t + 2, j.n_pre - 1)); }
+                f32x4 s[NS][RT];
+                scores(buf, s);
+                const int live = j.len - t * KT;
+                if (live < KT) {
+#pragma unroll
+                    for (int k = 0; k < NS; ++k)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            if (16 * k + 4 * g + x >= live)
+#pragma unroll
+                                for (int q = 0; q < RT; ++q) s[k][q][x] = -INFINITY;
+                }
+                st.template softmax<NS>(s, cc);
+                st.template add<NS, VROW>(s, lds + buf * (KBYTES + VBYTES) + KBYTES, g, r, T());
+                buf ^= 1;
+                if (more) store(buf, j.len - (t + 1) * KT);
+                __syncthreads();
+            }
+        }
+        if (j.t1 > j.n_pre) {                                                      // the drafted rows: one tile
+            load_tree();
+            int odd = 0;
+#pragma unroll
+            for (int x = 0; x < NL; ++x) odd |= Elem<T>::odd(rv[x]);
+            const bool any_odd = __syncthreads_or(odd);
+            if (any_odd)
+#pragma unroll
+                for (int x = 0; x < NL; ++x) rv[x] = finite_only(rv[x]);
+            store(buf, j.count);
+            __syncthreads();
+            f32x4 s[NS][RT];
+            scores(buf, s);
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) if (!((mask[q] >> (16 * k + 4 * g + x)) & 1)) s[k][q][x] = -INFINITY;
+            st.template softmax<NS>(s, cc);
+            st.template add<NS, VROW>(s, lds + buf * (KBYTES + VBYTES) + KBYTES, g, r, T());
+            if (any_odd) add_odd_values<T, D, RT, NS>(c, a, p, j, table, head_off, page_e, 0, s, mask, st, g, r);
+        }
+    }
+    const bool whole = j.pieces == 1;
+    float* part = whole ? nullptr : p.part + (((int64_t)j.slot * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (64 * RT) * (D + 2);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float l = st.l[t];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        const int at = row0 + t * 16 + r;
+        if (at >= rows) continue;
+        const int node = at / G;
+        if (whole) {
+            T* out = reinterpret_cast<T*>(a.d_out) + j.i * a.o_seq + node * a.o_node + (j.kh * G + at % G) * a.o_head;
+            const int kind = j.ok == 1 ? node >= j.count ? 0 : s_wrong[node] ? 2 : 1 : j.ok;
+            const float f = 1.f / l;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+                store4<T>(out + 16 * d + 4 * g, kind == 1 ? st.o[d][t] * f : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
+        } else {
+            float* to = part + (int64_t)(wid * RT * 16 + t * 16 + r) * (D + 2);
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                *reinterpret_cast<f32x2*>(to + 16 * d + 4 * g) = f32x2{st.o[d][t][0], st.o[d][t][1]};
+                *reinterpret_cast<f32x2*>(to + 16 * d + 4 * g + 2) = f32x2{st.o[d][t][2], st.o[d][t][3]};
+            }
+            if (g == 0) { to[D] = st.m[t]; to[D + 1] = j.ok == 2 ? __builtin_nanf("") : l; }
+        }
+    }
+}
+
+// ---- merge of the pieces of a sequence: grid (sequence, key / value head, row), D / 2 threads and more rows a workgroup ----------------
+template <typename T, int D, int KT>
+__global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
+    __shared__ int s_first, s_pieces, s_wrong[64];
+    const int i = blockIdx.x, kh = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const int seq = a.d_seqs[i];
     if (tid < 64) {
-        bool bad;
-        const uint64_t m = tree_mask(a.d_parents ? a.d_parents + (int64_t)i * a.n_nodes : nullptr, lane, a.n_nodes, &bad);
-        if (tid == node) { s_mask = m; s_bad = bad; }
-    }
-    T* out = reinterpret_cast<T*>(a.d_out) + i * a.o_seq + node * a.o_node + h * a.o_head;
-    __syncthreads();
-    if (node >= count && what == 1) what = 0;
-    if (what == 1 && s_bad) what = 2;
-    if (what != 1) {
-        for (int x = tid; x < D; x += 256) out[x] = (T)(what == 2 ? __builtin_nanf("") : 0.f);
-        return;
-    }
-    const T* q = reinterpret_cast<const T*>(a.d_q) + i * a.q_seq + node * a.q_node + h * a.q_head;
-    for (int x = tid; x < D; x += 256) sq[x] = (float)q[x] * a.scale;
-    __syncthreads();
-    const uint64_t mask = s_mask;
-    const int kh = h / (a.n_head / c.n_kv_head), PS = c.page_size;
-    const int32_t* row = c.d_table + (int64_t)a.d_seqs[i] * c.max_pages;
-    const int64_t page_e = (int64_t)c.n_kv_head * PS * D, layer_e = (int64_t)a.layer * c.n_pages * page_e;
-    const T* K = reinterpret_cast<const T*>(c.d_k) + layer_e + (int64_t)kh * PS * D;
-    const T* V = reinterpret_cast<const T*>(c.d_v) + layer_e + (int64_t)kh * PS * D;
-    float m = -INFINITY, l = 0.f, o[D];
+        // the first slot of sequence i: every earlier sequence's pieces
+        int per = p.per;
+        if (per == 0) {
+            int64_t all = 0;
+            for (int x = lane; x < a.n; x += 64) all += tree_tiles_of(c, a, p, x, KT);
 #pragma unroll
-    for (int x = 0; x < D; ++x) o[x] = 0.f;
-    for (int t = tid; t < len + count; t += 256) {
-        if (t >= len && !((mask >> (t - len)) & 1)) continue;
-        const int64_t off = row[t / PS] * page_e + (int64_t)(t % PS) * D;
-        float s = 0.f;
-#pragma unroll
-        for (int x = 0; x < D; x += E) {
-            float v[E];
-            load_f32(K + off + x, v);
-#pragma unroll
-            for (int j = 0; j < E; ++j) s = fmaf(sq[x + j], v[j], s);
+            for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
+            per = (int)max((int64_t)p.least, (all * c.n_kv_head * p.row_blocks + p.target - 1) / p.target);
         }
-        const float mn = fmaxf(m, s), al = m == -INFINITY ? 0.f : expf(m - mn), p = expf(s - mn);
-        m = mn; l = l * al + p;
+        int before = 0;
+        for (int x = lane; x < i; x += 64) before += (tree_tiles_of(c, a, p, x, KT) + per - 1) / per;
 #pragma unroll
-        for (int x = 0; x < D; x += E) {
-            float v[E];
-            load_f32(V + off + x, v);
-#pragma unroll
-            for (int j = 0; j < E; ++j) o[x + j] = fmaf(p, v[j], o[x + j] * al);
-        }
-    }
-    red[tid] = m;
-    __syncthreads();
-    float M = -INFINITY;
-    for (int t = 0; t < 256; ++t) M = fmaxf(M, red[t]);
-    const float f = m == -INFINITY ? 0.f : expf(m - M);
-    __syncthreads();
-    red[tid] = l * f;
-    __syncthreads();
-    float L = 0.f;
-    for (int t = 0; t < 256; ++t) L += red[t];
-    for (int x = 0; x < D; ++x) {
-        float v = o[x] * f;
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
-        if (lane == 0) so[tid >> 6][x] = v;
+        for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off);
+        bool wrong;
+        (void)tree_mask(a.d_parents ? a.d_parents + (int64_t)i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
+        s_wrong[lane] = wrong;
+        if (lane == 0) { s_first = before; s_pieces = (tree_tiles_of(c, a, p, i, KT) + per - 1) / per; }
     }
     __syncthreads();
-    for (int x = tid; x < D; x += 256) out[x] = (T)((so[0][x] + so[1][x] + so[2][x] + so[3][x]) / L);
+    const int pieces = s_pieces, first = s_first;
+    if (pieces <= 1) return;                                                        // written by the piece itself
+    const int count = a.d_counts ? min(max(a.d_counts[i], 0), a.n_nodes) : a.n_nodes;
+    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G;
+    const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
+    constexpr int TPR = D / 4, RPB = 256 / TPR;
+    const int row = blockIdx.z * RPB + tid / TPR, x = (tid % TPR) * 4;
+    if (row >= rows) return;
+    const int node = row / G;
+    const int64_t step = (int64_t)c.n_kv_head * p.row_blocks * p.rows * (D + 2);
+    const float* part = p.part + ((((int64_t)first * c.n_kv_head + kh) * p.row_blocks + row / p.rows) * p.rows + row % p.rows) * (D + 2);
+    float M = -INFINITY, L = 0.f;
+    for (int q = 0; q < pieces; ++q) M = fmaxf(M, part[q * step + D]);
+    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < pieces; ++q) {
+        const float* from = part + q * step;
+        const float m = from[D], f = m == M ? 1.f : __builtin_amdgcn_exp2f((m - M) * cc);
+        L = fmaf(from[D + 1], f, L);
+        const f32x2 lo = *reinterpret_cast<const f32x2*>(from + x), hi = *reinterpret_cast<const f32x2*>(from + x + 2);
+        v += f32x4{lo[0], lo[1], hi[0], hi[1]} * f;
+    }
+    T* out = reinterpret_cast<T*>(a.d_out) + i * a.o_seq + node * a.o_node + (kh * G + row % G) * a.o_head + x;
+    const int kind = seq == -1 || node >= count ? 0 : s_wrong[node] ? 2 : 1;
+    store4<T>(out, kind == 1 ? v * (1.f / L) : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
+}
+
+// Which kernel, and how the work is cut.
+struct TreeForm { bool rows_form; int rt, rows, kt; };
+static TreeForm tree_form(const wx_cache& c, const wx_tree_attn& a) {
+    const int rows = a.n_nodes * (a.n_head / c.n_kv_head), es = c.precision == WX_PREC_F32 ? 4 : 2;
+    TreeForm f;
+    f.rows_form = c.precision == WX_PREC_BF16 && rows > 32;
+    f.rt = f.rows_form ? rows > 64 ? 2 : 1 : rows > 16 ? 2 : 1;
+    f.rows = f.rows_form ? 64 * f.rt : 16 * f.rt;
+    f.kt = f.rows_form ? 64 : 8192 / (c.head_dim * es);
+    return f;
+}
+static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeForm& f) {
+    TreePlan p{};
+    const int rows = a.n_nodes * (a.n_head / c.n_kv_head);
+    p.row_blocks = (rows + f.rows - 1) / f.rows;
+    p.rows = f.rows;
+    p.tree_tiles = (a.n_nodes + f.kt - 1) / f.kt;
+    while ((1 << p.shift) < c.page_size) ++p.shift;
+    const int64_t most = ((int64_t)c.max_pages * c.page_size + f.kt - 1) / f.kt + p.tree_tiles;       // tiles of the longest sequence the tables hold
+    const int64_t units = (int64_t)c.n_kv_head * p.row_blocks;
+    p.least = 512 / f.kt + p.tree_tiles;
+    p.target = f.rows_form ? 512 : 768;
+    if (a.split_tokens > 0) {                                                       // at most 256 pieces a sequence
+        p.per = (int)(((int64_t)a.split_tokens + f.kt - 1) / f.kt);
+        if (p.per < (most + 255) / 256) p.per = (int)((most + 255) / 256);
+    }
+    p.single = most <= (p.per ? p.per : p.least);
+    if (p.single) p.slots = a.n;
+    else if (p.per) p.slots = (int)(a.n * ((most + p.per - 1) / p.per));
+    else p.slots = (int)(a.n + (p.target + units - 1) / units);
+    return p;
+}
+static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {
+    return p.single ? 0 : (int64_t)p.slots * c.n_kv_head * p.row_blocks * p.rows * (c.head_dim + 2) * 4;
 }
 
 // ---- verification ---------------------------------------------------------------------------------------------------------------------
@@ -251,7 +920,7 @@ extern "C" {
 
 int64_t wx_tree_attention_work_bytes(const wx_cache* c, const wx_tree_attn* a) {
     if (const char* m = tree_fault(c, a)) return set_error(WX_ERR_INVALID, m);
-    return 0;
+    return tree_part_bytes(*c, tree_plan(*c, *a, tree_form(*c, *a)));
 }
 
 int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
@@ -266,18 +935,37 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
     if (((uintptr_t)a->d_q | (uintptr_t)a->d_out | (uintptr_t)a->d_kn | (uintptr_t)a->d_vn) & 15) return set_error(WX_ERR_INVALID, "rows must be 16-byte aligned");
     OnDevice on(c->device);
     hipStream_t st = (hipStream_t)stream;
-    if (a->d_kn) {
-        const int64_t ks[4] = {0, a->kn_seq, a->kn_node, a->kn_head}, vs[4] = {0, a->vn_seq, a->vn_node, a->vn_head};
-        const int r = wx_cache_append(c, a->d_seqs, a->d_counts, a->n, a->n_nodes, a->layer, 1, a->d_kn, ks, a->d_vn, vs, stream);
-        if (r) return r;
-    }
-    const dim3 grid(a->n_nodes, a->n_head, a->n), block(256);
-    if (c->precision == WX_PREC_F32) {
-        if (c->head_dim == 64) hipLaunchKernelGGL((tree_attention_kernel<float, 64>), grid, block, 0, st, *c, *a);
-        else hipLaunchKernelGGL((tree_attention_kernel<float, 128>), grid, block, 0, st, *c, *a);
+    const TreeForm f = tree_form(*c, *a);
+    TreePlan p = tree_plan(*c, *a, f);
+    p.part = (float*)a->d_work;
+    const int64_t need = tree_part_bytes(*c, p);
+    if (need > 0 && (!a->d_work || a->work_bytes < need || ((uintptr_t)a->d_work & 15))) return set_error(WX_ERR_INVALID, "work buffer too small or not 16-byte aligned");
+    const int64_t jobs = ((int64_t)p.slots * c->n_kv_head + 7) / 8 * 8 * p.row_blocks;
+    if (jobs > 0x7fffffff) return set_error(WX_ERR_INVALID, "too many pieces: larger split_tokens, or fewer sequences");
+    const dim3 grid((unsigned)jobs), block(256);
+    const bool f32 = c->precision == WX_PREC_F32, wide = c->head_dim == 128;
+#define TREE_KEYS(T, D, RT) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT>), grid, block, 0, st, *c, *a, p)
+#define TREE_ROWS(D, RT) hipLaunchKernelGGL((tree_attention_rows_kernel<D, RT>), grid, block, 0, st, *c, *a, p)
+    if (f.rows_form) {
+        if (wide) { if (f.rt == 2) TREE_ROWS(128, 2); else TREE_ROWS(128, 1); }
+        else { if (f.rt == 2) TREE_ROWS(64, 2); else TREE_ROWS(64, 1); }
+    } else if (f32) {
+        if (wide) { if (f.rt == 2) TREE_KEYS(float, 128, 2); else TREE_KEYS(float, 128, 1); }
+        else { if (f.rt == 2) TREE_KEYS(float, 64, 2); else TREE_KEYS(float, 64, 1); }
     } else {
-        if (c->head_dim == 64) hipLaunchKernelGGL((tree_attention_kernel<bf16, 64>), grid, block, 0, st, *c, *a);
-        else hipLaunchKernelGGL((tree_attention_kernel<bf16, 128>), grid, block, 0, st, *c, *a);
+        if (wide) { if (f.rt == 2) TREE_KEYS(bf16, 128, 2); else TREE_KEYS(bf16, 128, 1); }
+        else { if (f.rt == 2) TREE_KEYS(bf16, 64, 2); else TREE_KEYS(bf16, 64, 1); }
+    }
+    if (!p.single) {
+        const int rows = a->n_nodes * (a->n_head / c->n_kv_head), rpb = 1024 / c->head_dim;
+        const dim3 mg(a->n, c->n_kv_head, (rows + rpb - 1) / rpb);
+        if (f32) {
+            if (wide) hipLaunchKernelGGL((tree_attention_merge_kernel<float, 128, 16>), mg, block, 0, st, *c, *a, p);
+            else hipLaunchKernelGGL((tree_attention_merge_kernel<float, 64, 32>), mg, block, 0, st, *c, *a, p);
+        } else if (f.kt == 64) {
+            if (wide) hipLaunchKernelGGL((tree_attention_merge_kernel<bf16, 128, 64>), mg, block, 0, st, *c, *a, p);
+            else hipLaunchKernelGGL((tree_attention_merge_kernel<bf16, 64, 64>), mg, block, 0, st, *c, *a, p);
+        } else hipLaunchKernelGGL((tree_attention_merge_kernel<bf16, 128, 32>), mg, block, 0, st, *c, *a, p);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? WX_OK : set_error(WX_ERR_HIP, hipGetErrorString(e));
