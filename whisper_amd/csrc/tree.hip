@@ -5,22 +5,28 @@
 //   pick_i = arg max_x logit_i[x],   log p(pick_i) = -log sum_x exp(logit_i[x] - max)
 #include "common.h"
 
+#include <atomic>
+
 namespace wx {
 
 constexpr int TR_NODES = 64;              // nodes a sequence: one bit each of a mask
 constexpr float TR_LOG2E = 1.4426950408889634f;
 
-// How the committed tokens of a batch are cut into pieces that workgroups take side by side.  A sequence has ceil(len / KT) tiles of
-// committed tokens and `tree_tiles` behind them; a piece is at most `per` tiles.  per == 0: by the batch, so that about `target`
-// pieces come out (one round of workgroups over the chip), but not below `least` tiles, which keeps a merge worth its traffic.
+// How the work on a batch is cut.  A sequence has ceil(len / KT) tiles of committed tokens and `tree_tiles` behind them.  For every
+// key / value head and block of rows, `takers` workgroups take equal shares of all sequences' tiles in a row (fewer takers where a
+// share would fall below `least` tiles), so that ragged lengths leave no workgroup behind: one may end a sequence, do some whole ones
+// and begin another.  The part of a sequence that taker w does is piece w + i of the part buffer (w or i grows by one from piece to
+// piece, so the numbers are distinct).  With `per` > 0 a sequence is cut into pieces of at most `per` tiles instead, one for each
+// workgroup; with `single`, where no sequence can be longer than `least` tiles, a workgroup does one whole sequence.
 struct TreePlan {
     int row_blocks;          // workgroups over the rows (nodes x query heads of a key / value head)
-    int tree_tiles, per, least, target;
-    int single;              // 1: no sequence that the tables can hold has a second piece
+    int tree_tiles, per, least, takers;
+    int single;              // (the kernels' ONE)
     int shift;               // log2 of the page size
-    int slots;               // pieces x sequences that the grid has room for
+    int slots;               // workgroups for each key / value head and block of rows
+    int pieces;              // ... and places for their parts
     int rows;                // rows a workgroup
-    float* part;             // [slots][n_kv_head][row_blocks][rows][D + 2]: output, maximum and sum of a piece (more than one piece only)
+    float* part;             // [pieces][n_kv_head][row_blocks][rows][D + 2]: output, maximum and sum (sequences in more than one piece)
 };
 
 __device__ __forceinline__ int tree_tiles_of(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, int i, int kt) {
@@ -28,76 +34,114 @@ __device__ __forceinline__ int tree_tiles_of(const wx_cache& c, const wx_tree_at
     const int len = s >= 0 && s < c.max_seqs ? min(max(c.d_lens[s], 0), c.max_pages << p.shift) : 0;
     return (len + kt - 1) / kt + p.tree_tiles;
 }
-// one wave: the sequence and piece that slot g stands for, how many pieces the sequence has and its first slot; false: none
-__device__ __forceinline__ bool tree_locate(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, int kt, int g, int lane, int* seq, int* piece, int* pieces) {
-    if (p.single) { *seq = g; *piece = 0; *pieces = 1; return g < a.n; }
-    int per = p.per;
-    if (per == 0) {
-        int64_t all = 0;
-        for (int i = lane; i < a.n; i += 64) all += tree_tiles_of(c, a, p, i, kt);
+// the share that tile x of `all` falls to (share w: tiles w * all / takers and up)
+__device__ __forceinline__ int tree_taker(int64_t x, int64_t all, int takers) { return (int)(((x + 1) * takers - 1) / all); }
+
+// One wave, all lanes alike: tiles of the whole batch, and how many takers they are for.
+__device__ __forceinline__ int64_t tree_all(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, int kt, int lane, int* takers) {
+    int64_t all = 0;
+    for (int i = lane; i < a.n; i += 64) all += tree_tiles_of(c, a, p, i, kt);
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
-        const int64_t units = (int64_t)c.n_kv_head * p.row_blocks;
-        per = (int)max((int64_t)p.least, (all * units + p.target - 1) / p.target);
-    }
-    int first = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 64) {
-        const int i = i0 + lane;
-        const int mine = i < a.n ? (tree_tiles_of(c, a, p, i, kt) + per - 1) / per : 0;
-        int upto = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) { const int u = __shfl_up(upto, off); if (lane >= off) upto += u; }
-        const uint64_t past = __ballot(first + upto > g);
-        if (past) {
-            const int at = __ffsll((unsigned long long)past) - 1;
-            *seq = i0 + at;
-            *pieces = __shfl(mine, at);
-            *piece = g - (first + __shfl(upto, at) - *pieces);
-            return true;
-        }
-        first += __shfl(upto, 63);
-    }
-    return false;
+    for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
+    *takers = (int)max((int64_t)1, min((int64_t)p.takers, all / p.least));
+    return all;
 }
 
-// What a workgroup has to do: sequence entry i, key / value head, block of rows, tiles [t0, t1) of the sequence's n_pre + tree_tiles.
+// What a workgroup has to do now: sequence entry i, key / value head, block of rows, tiles [t0, t1) of the sequence's n_pre + tree_tiles.
 struct TreeJob {
-    int ok;                  // 0: the rows are 0 (padding, no nodes), 1: attend, 2: refused (NaN)
-    int i, kh, rb, slot, piece, pieces, seq, len, count, n_pre, t0, t1, last;
+    int ok;                  // 0: the rows are 0 (padding, no nodes), 1: attend, 2: refused (NaN), -1: nothing (any more)
+    int i, kh, rb, piece, whole, seq, len, count, n_pre, t0, t1, last;
+    int w, takers;           // shares
+    int64_t all, start, x0, x1;   // tiles of the batch; first tile of sequence i among them; the share
 };
 
-template <int KT>
-__device__ __forceinline__ bool tree_job(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob* sh, TreeJob& j) {
-    // XCD-aware: consecutive workgroups go to different XCDs, so the row blocks that read the same keys are 8 apart, on one L2
-    const int units = c.n_kv_head, lin = blockIdx.x, x = lin % 8, y = lin / 8;
-    const int w = (y / p.row_blocks) * 8 + x;
-    const int tid = threadIdx.x, slot = w / units;
-    if (slot >= p.slots) return false;
+__device__ __forceinline__ void tree_fill(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, int kt, TreeJob& t) {
+    t.ok = 1;
+    t.seq = a.d_seqs[t.i];
+    t.count = a.d_counts ? min(max(a.d_counts[t.i], 0), a.n_nodes) : a.n_nodes;
+    t.len = 0; t.n_pre = 0;
+    if (t.seq == -1) t.ok = 0;
+    else if (t.seq < 0 || t.seq >= c.max_seqs) t.ok = 2;
+    else {
+        t.len = c.d_lens[t.seq];
+        if (t.len < 0 || (int64_t)t.len + t.count > (int64_t)min(c.d_held[t.seq], c.max_pages) << p.shift) t.ok = 2;
+        else if (t.count == 0) t.ok = 0;
+        t.n_pre = (min(max(t.len, 0), c.max_pages << p.shift) + kt - 1) / kt;
+    }
+}
+
+// The first job of a workgroup (first = true) or the next of its share; *sh is the same on every thread afterwards.
+template <int KT, bool ONE>
+__device__ __forceinline__ bool tree_next(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob* sh, TreeJob& j, bool first) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (!first && (ONE || p.per)) return false;
+    __syncthreads();                                               // the job before is done with *sh and the other shared arrays
     if (tid < 64) {
-        int seq = 0, piece = 0, pieces = 0;
-        const bool any = tree_locate(c, a, p, KT, slot, tid, &seq, &piece, &pieces);
-        if (tid == 0) {
-            TreeJob t;
-            t.ok = any ? 1 : -1; t.i = seq; t.kh = w % units; t.rb = y % p.row_blocks; t.slot = slot; t.piece = piece; t.pieces = pieces;
-            t.seq = 0; t.len = 0; t.count = 0; t.n_pre = 0; t.t0 = 0; t.t1 = 0; t.last = 0;
-            if (any) {
-                t.seq = a.d_seqs[seq];
-                t.count = a.d_counts ? min(max(a.d_counts[seq], 0), a.n_nodes) : a.n_nodes;
-                if (t.seq == -1) t.ok = 0;
-                else if (t.seq < 0 || t.seq >= c.max_seqs) t.ok = 2;
-                else {
-                    t.len = c.d_lens[t.seq];
-                    if (t.len < 0 || (int64_t)t.len + t.count > (int64_t)min(c.d_held[t.seq], c.max_pages) << p.shift) t.ok = 2;
-                    else if (t.count == 0) t.ok = 0;
-                    t.n_pre = (min(max(t.len, 0), c.max_pages << p.shift) + KT - 1) / KT;
-                    const int all = t.n_pre + p.tree_tiles, per = (all + pieces - 1) / pieces;
-                    t.t0 = min(all, piece * per); t.t1 = min(all, t.t0 + per);
-                    if (t.t0 == t.t1) t.t0 = t.t1 = 0;                              // a piece may be left without tiles
-                    t.last = t.t1 == all;
+        TreeJob t;
+        if (first) {
+            // XCD-aware: consecutive workgroups go to different XCDs, so the row blocks that read the same keys are 8 apart, on one L2
+            const int lin = blockIdx.x, y = lin / 8, w = (y / p.row_blocks) * 8 + lin % 8;
+            t.kh = w % c.n_kv_head; t.rb = y % p.row_blocks; t.w = w / c.n_kv_head; t.whole = 1; t.piece = 0; t.i = t.w; t.takers = 0;
+            t.all = t.start = t.x0 = t.x1 = 0;
+            t.ok = t.w < p.slots ? 1 : -1;
+            if (t.ok == 1 && !ONE) {
+                if (p.per) {                                       // piece number t.w, counted through the sequences
+                    int before = 0;
+                    t.ok = -1;
+                    for (int i0 = 0; i0 < a.n && t.ok < 0; i0 += 64) {
+                        const int i = i0 + lane, mine = i < a.n ? (tree_tiles_of(c, a, p, i, KT) + p.per - 1) / p.per : 0;
+                        int upto = mine;
+#pragma unroll
+                        for (int off = 1; off < 64; off <<= 1) { const int u = __shfl_up(upto, off); if (lane >= off) upto += u; }
+                        const uint64_t past = __ballot(before + upto > t.w);
+                        if (past) {
+                            const int at = __ffsll((unsigned long long)past) - 1, pieces = __shfl(mine, at);
+                            t.ok = 1; t.i = i0 + at; t.whole = pieces == 1; t.piece = t.w;
+                            const int q = t.w - (before + __shfl(upto, at) - pieces);
+                            t.x0 = (int64_t)q * p.per; t.x1 = t.x0 + p.per;
+                        }
+                        before += __shfl(upto, 63);
+                    }
+                } else {                                           // share number t.w: the sequence of its first tile
+                    t.all = tree_all(c, a, p, KT, lane, &t.takers);
+                    if (t.w >= t.takers) t.ok = -1;
+                    t.x0 = t.w * t.all / t.takers; t.x1 = (t.w + (int64_t)1) * t.all / t.takers;
+                    for (int i0 = 0; i0 < a.n && t.ok == 1; i0 += 64) {
+                        const int i = i0 + lane;
+                        int64_t upto = i < a.n ? tree_tiles_of(c, a, p, i, KT) : 0;
+                        const int64_t mine = upto;
+#pragma unroll
+                        for (int off = 1; off < 64; off <<= 1) { const int64_t u = __shfl_up(upto, off); if (lane >= off) upto += u; }
+                        const uint64_t past = __ballot(t.start + upto > t.x0);
+                        if (past) {
+                            const int at = __ffsll((unsigned long long)past) - 1;
+                            t.i = i0 + at;
+                            t.start += __shfl(upto - mine, at);
+                            break;
+                        }
+                        t.start += __shfl(upto, 63);
+                    }
                 }
             }
-            *sh = t;
+        } else {
+            t = *sh;
+            t.start += t.n_pre + p.tree_tiles;
+            t.i += 1;
+            t.ok = t.i < a.n && t.start < t.x1 ? 1 : -1;
         }
+        if (t.ok == 1) {
+            tree_fill(c, a, p, KT, t);
+            const int tiles = t.n_pre + p.tree_tiles;
+            if (ONE) { t.t0 = 0; t.t1 = tiles; }
+            else if (p.per) { t.t0 = (int)t.x0; t.t1 = (int)min(t.x1, (int64_t)tiles); }
+            else {
+                t.t0 = (int)max((int64_t)0, t.x0 - t.start); t.t1 = (int)min((int64_t)tiles, t.x1 - t.start);
+                t.whole = tree_taker(t.start, t.all, t.takers) == tree_taker(t.start + tiles - 1, t.all, t.takers);
+                t.piece = t.w + t.i;
+            }
+            t.last = t.t1 == tiles;
+        }
+        if (tid == 0) *sh = t;
     }
     __syncthreads();
     j = *sh;
@@ -106,16 +150,15 @@ __device__ __forceinline__ bool tree_job(const wx_cache& c, const wx_tree_attn& 
     if (j.ok == 1) {
         // the pages of this piece's tiles (of the draft's rows too, which have to be this slot's alone where they are written)
         const int32_t* row = c.d_table + (int64_t)j.seq * c.max_pages;
-        const bool tail = j.t1 > j.n_pre;
-        const int upto = tail ? j.len + j.count : min(j.len, j.t1 * KT);
+        const int upto = j.t1 > j.n_pre ? j.len + j.count : min(j.len, j.t1 * KT);
         const int own = a.d_kn && j.last ? j.len >> p.shift : 0x7fffffff;
-        for (int q = (min(j.t0 * KT, j.len) >> p.shift) + tid; q << p.shift < upto; q += 256) {
+        for (int q = (min(j.t0 * KT, j.len) >> p.shift) + tid; q << p.shift < upto; q += blockDim.x) {
             const int page = row[q];
             if ((unsigned)page >= (unsigned)c.n_pages || (q >= own && c.d_refs[page] != 1)) bad = 1;
         }
-        if (a.d_kn) for (int k = tid; k < j.i; k += 256) bad |= a.d_seqs[k] == j.seq;
+        if (a.d_kn) for (int k = tid; k < j.i; k += blockDim.x) bad |= a.d_seqs[k] == j.seq;
     }
-    if (__syncthreads_or(bad)) j.ok = 2;
+    if (__syncthreads_or(bad)) { j.ok = 2; if (tid == 0) sh->ok = 2; }             // (read again behind the caller's next barrier)
     return true;
 }
 
@@ -321,7 +364,7 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // Bound by the stream of keys and values.  A tile is 8 KiB of keys (straight into the matrix instruction's registers) and 8 KiB of
 // values (through the wave's own LDS, for the transposing read); the next tile's 16 loads a lane are issued as soon as the scores of
 // this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
-template <typename T, int D, int RT>
+template <typename T, int D, int RT, bool ONE>
 __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
     typedef typename Elem<T>::Frag Frag;
     constexpr int E = 16 / sizeof(T), KT = 8192 / (D * (int)sizeof(T)), NS = KT / 16, KS = D / (4 * E), CPR = D / E, NV = KT * CPR / 64;
@@ -334,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c,
     __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, r = lane & 15;
     TreeJob j;
-    if (!tree_job<KT>(c, a, p, &s_job, j)) return;
+    for (bool first = true; tree_next<KT, ONE>(c, a, p, &s_job, j, first); first = false) {
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * RT * 16;
     if (wid == 0 && j.ok == 1) {
         bool wrong;
@@ -438,6 +481,7 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c,
                     ids = load_ids(min(t + 8, j.n_pre - 1));
                 }
                 if (live < KT) {
+                    asm volatile("");                                               // keep it a branch: as selects it costs every tile
 #pragma unroll
                     for (int k = 0; k < NS; ++k)
 #pragma unroll
@@ -487,8 +531,8 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c,
         if (g == 0) { s_m[wid][t * 16 + r] = st.m[t]; s_l[wid][t * 16 + r] = l; }
     }
     __syncthreads();
-    const bool whole = j.pieces == 1;
-    float* part = whole ? nullptr : p.part + (((int64_t)j.slot * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (RT * 16) * (D + 2);
+    const bool whole = j.whole;
+    float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (RT * 16) * (D + 2);
     const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
     float f[RT];
 #pragma unroll
@@ -538,46 +582,62 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c,
             }
         }
     }
+    }
 }
 
 // ---- many rows (bf16): every wave has rows of its own, the workgroup shares the tiles of keys and values ------------------------------
-// Bound by the matrix pipe and the softmax between its two products.  Tiles of 64 keys are loaded into registers while the tile before
-// is worked on, and go to a double-buffered LDS image (one barrier a tile).
-template <int D, int RT>
-__global__ __launch_bounds__(256, 2) void tree_attention_rows_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
+// Eight waves, RT x 16 rows each (two waves on every SIMD of a CU).  Tiles of 64 keys go from HBM to LDS without registers
+// (global_load_lds) into a ring of four, two to three tiles ahead; a wave-instruction writes 1 KiB of rows in a line, so the swizzle
+// that the fragment reads need (16-byte chunk x of a row in slot x ^ (row mod chunks)) is applied to its lanes' source addresses.
+// The softmax of a tile takes the vector pipe about as long as its two products take the matrix pipe.  So waves 4-7 run half a tile
+// behind waves 0-3, a barrier each half: while one wave of a SIMD does PV(t - 1) and QK(t), the other does the softmax of its tile.
+//
+// 16 bytes a lane from global memory to LDS address `to` + 16 x lane (alike on the wave).  Written out because the compiler, which knows
+// of the builtin's LDS write, waits for ALL loads before every transposing LDS read, whatever they write; the waits are the kernel's own.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"                            // m0 is named as changed on purpose
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(to) : "m0", "memory");
+}
+#pragma clang diagnostic pop
+typedef const __attribute__((address_space(4))) int32_t const_i32;        // page numbers that are alike on a wave, by scalar loads
+constexpr int TRW = 8;                                                    // waves
+
+template <int D, int RT, bool ONE>
+__global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
     typedef bf16 T;
     typedef bf16x8 Frag;
-    constexpr int KT = 64, NS = 4, KS = D / 32, CPR = D / 8, NL = KT * CPR / 256;
-    constexpr int KROW = D * 2, VROW = D * 2 + 32, KBYTES = KT * KROW, VBYTES = KT * VROW;
-    __shared__ __attribute__((aligned(16))) char lds[2 * (KBYTES + VBYTES)];
+    constexpr int KT = 64, NS = 4, KS = D / 32, CPR = D / 8, ROWB = D * 2, HALF = KT * ROWB, RING = 4;
+    constexpr int RPW = KT / TRW, NL = RPW * CPR / 64, RPL = 64 / CPR;      // rows of a tile a wave brings, its loads for keys (values: as many), rows a load
+    extern __shared__ __attribute__((aligned(1024))) char lds[];            // RING x (keys, values)
     __shared__ TreeJob s_job;
     __shared__ uint64_t s_mask[64];
     __shared__ int s_wrong[64];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, r = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
+    const bool late = wid >= TRW / 2;
     TreeJob j;
-    if (!tree_job<KT>(c, a, p, &s_job, j)) return;
-    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * 64 * RT + wid * 16 * RT;
+    for (bool first = true; tree_next<KT, ONE>(c, a, p, &s_job, j, first); first = false) {
+    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * TRW * 16 * RT + wid * 16 * RT;
     if (wid == 0 && j.ok == 1) {
         bool wrong;
         const uint64_t m = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
         s_mask[lane] = m; s_wrong[lane] = wrong;
     }
     __syncthreads();
-    const int32_t* table = c.d_table + (int64_t)j.seq * c.max_pages;
-    const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)j.kh * c.page_size * D;
+    const int seq = __builtin_amdgcn_readfirstlane(j.seq), kh = __builtin_amdgcn_readfirstlane(j.kh), len = __builtin_amdgcn_readfirstlane(j.len);
+    const int32_t* table = c.d_table + (int64_t)seq * c.max_pages;
+    const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)kh * c.page_size * D;
     RowState<D, RT> st;
     st.init();
     const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
     if (j.ok == 1) {
         if (a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
         Frag qf[RT][KS];
-        uint64_t mask[RT];
         const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const int row = min(row0 + t * 16 + r, rows - 1), node = row / G;
-            const T* q = reinterpret_cast<const T*>(a.d_q) + j.i * a.q_seq + node * a.q_node + (j.kh * G + row % G) * a.q_head;
-            mask[t] = s_mask[node];
+            const T* q = reinterpret_cast<const T*>(a.d_q) + j.i * a.q_seq + node * a.q_node + (kh * G + row % G) * a.q_head;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 qf[t][ks] = *reinterpret_cast<const Frag*>(q + (ks * 4 + g) * 8);
@@ -589,73 +649,121 @@ __global__ __launch_bounds__(256, 2) void tree_attention_rows_kernel(wx_cache c,
         }
         const T* Kp = reinterpret_cast<const T*>(c.d_k) + head_off;
         const T* Vp = reinterpret_cast<const T*>(c.d_v) + head_off;
-        Frag rk[NL], rv[NL];
-        int ids[NL];
-        const int st_row = tid / CPR, st_ch = tid % CPR;                            // load p: row st_row + p * (256 / CPR)
-        constexpr int RPL = 256 / CPR;
-        auto load_ids = [&](int t) {
-#pragma unroll
-            for (int x = 0; x < NL; ++x) ids[x] = table[min(t * KT + st_row + x * RPL, j.len - 1) >> p.shift];
-        };
-        auto load_pre = [&](int t) {
-#pragma unroll
-            for (int x = 0; x < NL; ++x) {
-                const int at = min(t * KT + st_row + x * RPL, j.len - 1);
-                const int64_t off = ids[x] * page_e + (int64_t)(at & (c.page_size - 1)) * D + st_ch * 8;
-                rk[x] = *reinterpret_cast<const Frag*>(Kp + off);
-                rv[x] = *reinterpret_cast<const Frag*>(Vp + off);
-            }
-        };
-        auto load_tree = [&]() {
+        const int t0 = __builtin_amdgcn_readfirstlane(j.t0), n_tiles = __builtin_amdgcn_readfirstlane(min(j.t1, j.n_pre)) - t0;
+        const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
+        const const_i32* ctable = (const const_i32*)(uintptr_t)table;
+        // this wave's rows of tile t (all on one page: RPW divides 16) -> its place in the ring
+        auto page_of = [&](int t) { return ctable[min((t0 + t) * KT + wid * RPW, len - 1) >> p.shift]; };
+        auto issue = [&](int t, int page) {
+            const int64_t base = (int64_t)page * page_e;
+            const uint32_t to = lds0 + (t & (RING - 1)) * 2 * HALF + wid * RPW * ROWB;
 #pragma unroll
             for (int x = 0; x < NL; ++x) {
-                const int node = min(st_row + x * RPL, j.count - 1);
-                rk[x] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, true, node) + st_ch * 8);
-                rv[x] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, false, node) + st_ch * 8);
+                const int row = wid * RPW + x * RPL + lane / CPR, at = min((t0 + t) * KT + row, len - 1);
+                const int64_t off = base + (int64_t)(at & (c.page_size - 1)) * D + ((lane % CPR) ^ (row & (CPR - 1))) * 8;
+                load_to_lds(Kp + off, to + x * 1024);
+                load_to_lds(Vp + off, to + HALF + x * 1024);
             }
         };
-        // K image: chunk ch of row at slot ch ^ (row & 7): 16 rows' reads of one chunk hit every bank once
-        auto store = [&](int buf, int live) {
-            char* kb = lds + buf * (KBYTES + VBYTES);
+        // this wave's loads up to tile t are done (tile t + 1's, where there is one, may go on); rows past the last token count as 0 values
+        auto landed = [&](int t) {
+            if (t + 1 < n_tiles) {
+                if constexpr (NL == 2) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+                else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                const int live = len - (t0 + t) * KT;
+                if (live < KT) {
+                    char* vb = lds + (t & (RING - 1)) * 2 * HALF + HALF;
+                    for (int u = lane; u < RPW * CPR; u += 64) {
+                        const int row = wid * RPW + u / CPR;
+                        if (row >= live) *reinterpret_cast<Frag*>(vb + row * ROWB + (u % CPR) * 16) = Frag{};
+                    }
+                }
+            }
+        };
+        auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); __builtin_amdgcn_sched_barrier(0); };
+        // chunk 4 ks + g of key 16 k + r; chunk 2 d + (r & 3) / 2 of value row 32 h + 16 u + 4 g + r / 4
+        const int kx = (g ^ (r & (CPR - 1))) << 4, vrow = 4 * g + (r >> 2), vx = ((((r & 3) >> 1) ^ (vrow & (CPR - 1))) << 4);
+        // fragments of the next 16 keys (of the next 16 columns) are read while the matrix pipe works on these: the order is pinned, or the
+        // compiler reads each right before its use and waits for LDS every time
+        auto scores = [&](const char* kb, f32x4 (&s)[NS][RT]) {
+            Frag kf[2][KS];
+            auto read = [&](int k) {
 #pragma unroll
-            for (int x = 0; x < NL; ++x) {
-                const int row = st_row + x * RPL;
-                *reinterpret_cast<Frag*>(kb + row * KROW + ((st_ch ^ (row & 7)) << 4)) = rk[x];
-                *reinterpret_cast<Frag*>(kb + KBYTES + row * VROW + (st_ch << 4)) = row < live ? rv[x] : Frag{};
-            }
-        };
-        auto scores = [&](int buf, f32x4 (&s)[NS][RT]) {
-            const char* kb = lds + buf * (KBYTES + VBYTES);
+                for (int ks = 0; ks < KS; ++ks) kf[k & 1][ks] = *reinterpret_cast<const Frag*>(kb + (k * 16 + r) * ROWB + ((ks * 64) ^ kx));
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            read(0);
 #pragma unroll
             for (int k = 0; k < NS; ++k) {
-                const int row = k * 16 + r;
-                Frag kf[KS];
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const Frag*>(kb + row * KROW + (((ks * 4 + g) ^ (row & 7)) << 4));
+                if (k + 1 < NS) read(k + 1);
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
                     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) x = Elem<T>::qk(kf[ks], qf[t][ks], x);
+                    for (int ks = 0; ks < KS; ++ks) x = Elem<T>::qk(kf[k & 1][ks], qf[t][ks], x);
                     s[k][t] = x;
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        const int end = min(j.t1, j.n_pre);
-        int buf = 0;
-        if (j.t0 < end) {
-            load_ids(j.t0);
-            load_pre(j.t0);
-            load_ids(min(j.t0 + 1, j.n_pre - 1));
-            store(0, j.len - j.t0 * KT);
-            __syncthreads();
-            for (int t = j.t0; t < end; ++t) {
-                const bool more = t + 1 < end;
-                if (more) { load_pre(t + 1); load_ids(min(t + 2, j.n_pre - 1)); }
+        auto pack = [&](const f32x4 (&s)[NS][RT], Frag (&pf)[RT][2]) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) { pf[t][h][x] = (T)s[2 * h][t][x]; pf[t][h][4 + x] = (T)s[2 * h + 1][t][x]; }
+        };
+        auto add = [&](const char* vb, const Frag (&pf)[RT][2]) {
+            constexpr int AHEAD = 2;
+            Frag vf[AHEAD + 1][2];
+            auto read = [&](int d) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const char* p0 = vb + (32 * h + vrow) * ROWB + ((32 * d) ^ vx) + (r & 1) * 8;
+                    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0));
+                    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 16 * ROWB));
+                    vf[d % (AHEAD + 1)][h] = __builtin_bit_cast(Frag, (i16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+#pragma unroll
+            for (int d = 0; d < AHEAD; ++d) read(d);
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                if (d + AHEAD < D / 16) read(d + AHEAD);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) st.o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d % (AHEAD + 1)][h], pf[t][h], st.o[d][t], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        Frag pf[RT][2];
+        if (n_tiles > 0) {
+            __builtin_amdgcn_s_waitcnt(0);                                          // the counts below are of tiles' loads only (the builtin, so
+            __builtin_amdgcn_sched_barrier(0);                                      // that the compiler does not wait for the queries in the loop)
+            issue(0, page_of(0));
+            if (n_tiles > 1) issue(1, page_of(1));
+            int page = page_of(min(2, n_tiles - 1));
+            landed(0);
+            barrier();
+            if (late) barrier();
+            for (int t = 0; t < n_tiles; ++t) {
+                // the slot of tile t + 2 held tile t - 2, whose values the late waves read last, a barrier ago
+                if (t + 2 < n_tiles) { issue(t + 2, page); page = page_of(min(t + 3, n_tiles - 1)); }
+                __builtin_amdgcn_s_setprio(1);
+                if (t > 0) add(lds + ((t - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
                 f32x4 s[NS][RT];
-                scores(buf, s);
-                const int live = j.len - t * KT;
+                scores(lds + (t & (RING - 1)) * 2 * HALF, s);
+                __builtin_amdgcn_s_setprio(0);
+                if (late && t + 1 < n_tiles) landed(t + 1);
+                barrier();
+                const int live = len - (t0 + t) * KT;
                 if (live < KT) {
+                    asm volatile("");                                               // keep it a branch: as selects it costs every tile
 #pragma unroll
                     for (int k = 0; k < NS; ++k)
 #pragma unroll
@@ -665,25 +773,39 @@ __global__ __launch_bounds__(256, 2) void tree_attention_rows_kernel(wx_cache c,
                                 for (int q = 0; q < RT; ++q) s[k][q][x] = -INFINITY;
                 }
                 st.template softmax<NS>(s, cc);
-                st.template add<NS, VROW>(s, lds + buf * (KBYTES + VBYTES) + KBYTES, g, r, T());
-                buf ^= 1;
-                if (more) store(buf, j.len - (t + 1) * KT);
-                __syncthreads();
+                pack(s, pf);
+                if (!late && t + 1 < n_tiles) landed(t + 1);
+                barrier();
             }
+            add(lds + ((n_tiles - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
+            if (!late) barrier();
+            __syncthreads();
         }
-        if (j.t1 > j.n_pre) {                                                      // the drafted rows: one tile
-            load_tree();
+        j = s_job;                                                                 // not kept in registers over the loop
+        if (j.t1 > j.n_pre) {                                                      // the drafted rows: one tile, through registers
+            Frag rk[NL], rv[NL];
             int odd = 0;
 #pragma unroll
-            for (int x = 0; x < NL; ++x) odd |= Elem<T>::odd(rv[x]);
+            for (int x = 0; x < NL; ++x) {
+                const int node = min(wid * RPW + x * RPL + lane / CPR, j.count - 1);
+                rk[x] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, true, node) + (lane % CPR) * 8);
+                rv[x] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, false, node) + (lane % CPR) * 8);
+                odd |= Elem<T>::odd(rv[x]);
+            }
             const bool any_odd = __syncthreads_or(odd);
-            if (any_odd)
 #pragma unroll
-                for (int x = 0; x < NL; ++x) rv[x] = finite_only(rv[x]);
-            store(buf, j.count);
+            for (int x = 0; x < NL; ++x) {
+                const int row = wid * RPW + x * RPL + lane / CPR, slot = ((lane % CPR) ^ (row & (CPR - 1))) << 4;
+                if (any_odd) rv[x] = finite_only(rv[x]);
+                *reinterpret_cast<Frag*>(lds + row * ROWB + slot) = rk[x];
+                *reinterpret_cast<Frag*>(lds + HALF + row * ROWB + slot) = row < j.count ? rv[x] : Frag{};
+            }
             __syncthreads();
             f32x4 s[NS][RT];
-            scores(buf, s);
+            scores(lds, s);
+            uint64_t mask[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) mask[t] = s_mask[min(row0 + t * 16 + r, rows - 1) / G];
 #pragma unroll
             for (int k = 0; k < NS; ++k)
 #pragma unroll
@@ -691,12 +813,14 @@ __global__ __launch_bounds__(256, 2) void tree_attention_rows_kernel(wx_cache c,
 #pragma unroll
                     for (int q = 0; q < RT; ++q) if (!((mask[q] >> (16 * k + 4 * g + x)) & 1)) s[k][q][x] = -INFINITY;
             st.template softmax<NS>(s, cc);
-            st.template add<NS, VROW>(s, lds + buf * (KBYTES + VBYTES) + KBYTES, g, r, T());
+            pack(s, pf);
+            add(lds + HALF, pf);
             if (any_odd) add_odd_values<T, D, RT, NS>(c, a, p, j, table, head_off, page_e, 0, s, mask, st, g, r);
         }
     }
-    const bool whole = j.pieces == 1;
-    float* part = whole ? nullptr : p.part + (((int64_t)j.slot * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (64 * RT) * (D + 2);
+    j = s_job;
+    const bool whole = j.whole;
+    float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (TRW * 16 * RT) * (D + 2);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         float l = st.l[t];
@@ -722,6 +846,7 @@ __global__ __launch_bounds__(256, 2) void tree_attention_rows_kernel(wx_cache c,
             if (g == 0) { to[D] = st.m[t]; to[D + 1] = j.ok == 2 ? __builtin_nanf("") : l; }
         }
     }
+    }
 }
 
 // ---- merge of the pieces of a sequence: grid (sequence, key / value head, row), D / 2 threads and more rows a workgroup ----------------
@@ -731,23 +856,27 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
     const int i = blockIdx.x, kh = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int seq = a.d_seqs[i];
     if (tid < 64) {
-        // the first slot of sequence i: every earlier sequence's pieces
-        int per = p.per;
-        if (per == 0) {
-            int64_t all = 0;
-            for (int x = lane; x < a.n; x += 64) all += tree_tiles_of(c, a, p, x, KT);
+        int pieces, at;
+        if (p.per) {
+            int before = 0;
+            for (int x = lane; x < i; x += 64) before += (tree_tiles_of(c, a, p, x, KT) + p.per - 1) / p.per;
 #pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
-            per = (int)max((int64_t)p.least, (all * c.n_kv_head * p.row_blocks + p.target - 1) / p.target);
+            for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off);
+            pieces = (tree_tiles_of(c, a, p, i, KT) + p.per - 1) / p.per; at = before;
+        } else {
+            int takers;
+            const int64_t all = tree_all(c, a, p, KT, lane, &takers);
+            int64_t before = 0;
+            for (int x = lane; x < i; x += 64) before += tree_tiles_of(c, a, p, x, KT);
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off);
+            const int w = tree_taker(before, all, takers);
+            pieces = tree_taker(before + tree_tiles_of(c, a, p, i, KT) - 1, all, takers) - w + 1; at = w + i;
         }
-        int before = 0;
-        for (int x = lane; x < i; x += 64) before += (tree_tiles_of(c, a, p, x, KT) + per - 1) / per;
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off);
         bool wrong;
         (void)tree_mask(a.d_parents ? a.d_parents + (int64_t)i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
         s_wrong[lane] = wrong;
-        if (lane == 0) { s_first = before; s_pieces = (tree_tiles_of(c, a, p, i, KT) + per - 1) / per; }
+        if (lane == 0) { s_first = at; s_pieces = pieces; }
     }
     __syncthreads();
     const int pieces = s_pieces, first = s_first;
@@ -776,14 +905,28 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
     store4<T>(out, kind == 1 ? v * (1.f / L) : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
 }
 
+// (more LDS than a launch has by default: asked for once per device, before the first launch there)
+template <int D, int RT, bool ONE>
+static hipError_t launch_rows(dim3 grid, int lds, hipStream_t st, const wx_cache& c, const wx_tree_attn& a, const TreePlan& p) {
+    static std::atomic<uint64_t> asked{0};
+    const uint64_t bit = 1ull << (c.device & 63);
+    if (c.device > 63 || !(asked.load(std::memory_order_relaxed) & bit)) {
+        const hipError_t e = hipFuncSetAttribute((const void*)tree_attention_rows_kernel<D, RT, ONE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL((tree_attention_rows_kernel<D, RT, ONE>), grid, dim3(64 * TRW), lds, st, c, a, p);
+    return hipSuccess;
+}
+
 // Which kernel, and how the work is cut.
 struct TreeForm { bool rows_form; int rt, rows, kt; };
 static TreeForm tree_form(const wx_cache& c, const wx_tree_attn& a) {
     const int rows = a.n_nodes * (a.n_head / c.n_kv_head), es = c.precision == WX_PREC_F32 ? 4 : 2;
     TreeForm f;
-    f.rows_form = c.precision == WX_PREC_BF16 && rows > 32;
-    f.rt = f.rows_form ? rows > 64 ? 2 : 1 : rows > 16 ? 2 : 1;
-    f.rows = f.rows_form ? 64 * f.rt : 16 * f.rt;
+    f.rows_form = c.precision == WX_PREC_BF16 && rows > 64;
+    f.rt = f.rows_form ? rows > 128 ? 2 : 1 : rows > 16 ? 2 : 1;
+    f.rows = f.rows_form ? 128 * f.rt : 16 * f.rt;
     f.kt = f.rows_form ? 64 : 8192 / (c.head_dim * es);
     return f;
 }
@@ -797,19 +940,18 @@ static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeFo
     const int64_t most = ((int64_t)c.max_pages * c.page_size + f.kt - 1) / f.kt + p.tree_tiles;       // tiles of the longest sequence the tables hold
     const int64_t units = (int64_t)c.n_kv_head * p.row_blocks;
     p.least = 512 / f.kt + p.tree_tiles;
-    p.target = f.rows_form ? 512 : 768;
+    p.takers = (int)(((f.rows_form ? 256 : 768) + units - 1) / units);
     if (a.split_tokens > 0) {                                                       // at most 256 pieces a sequence
         p.per = (int)(((int64_t)a.split_tokens + f.kt - 1) / f.kt);
         if (p.per < (most + 255) / 256) p.per = (int)((most + 255) / 256);
     }
     p.single = most <= (p.per ? p.per : p.least);
-    if (p.single) p.slots = a.n;
-    else if (p.per) p.slots = (int)(a.n * ((most + p.per - 1) / p.per));
-    else p.slots = (int)(a.n + (p.target + units - 1) / units);
+    p.slots = p.single ? a.n : p.per ? (int)(a.n * ((most + p.per - 1) / p.per)) : p.takers;
+    p.pieces = p.single ? 0 : p.per ? p.slots : p.takers + a.n;
     return p;
 }
 static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {
-    return p.single ? 0 : (int64_t)p.slots * c.n_kv_head * p.row_blocks * p.rows * (c.head_dim + 2) * 4;
+    return (int64_t)p.pieces * c.n_kv_head * p.row_blocks * p.rows * (c.head_dim + 2) * 4;
 }
 
 // ---- verification ---------------------------------------------------------------------------------------------------------------------
@@ -944,8 +1086,11 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
     if (jobs > 0x7fffffff) return set_error(WX_ERR_INVALID, "too many pieces: larger split_tokens, or fewer sequences");
     const dim3 grid((unsigned)jobs), block(256);
     const bool f32 = c->precision == WX_PREC_F32, wide = c->head_dim == 128;
-#define TREE_KEYS(T, D, RT) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT>), grid, block, 0, st, *c, *a, p)
-#define TREE_ROWS(D, RT) hipLaunchKernelGGL((tree_attention_rows_kernel<D, RT>), grid, block, 0, st, *c, *a, p)
+#define TREE_KEYS(T, D, RT) do { if (p.single) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, true>), grid, block, 0, st, *c, *a, p); \
+                                 else hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, false>), grid, block, 0, st, *c, *a, p); } while (0)
+#define TREE_ROWS(D, RT) do { const int lds = 4 * 2 * 64 * D * 2; \
+                              const hipError_t le = p.single ? launch_rows<D, RT, true>(grid, lds, st, *c, *a, p) : launch_rows<D, RT, false>(grid, lds, st, *c, *a, p); \
+                              if (le != hipSuccess) return set_error(WX_ERR_HIP, hipGetErrorString(le)); } while (0)
     if (f.rows_form) {
         if (wide) { if (f.rt == 2) TREE_ROWS(128, 2); else TREE_ROWS(128, 1); }
         else { if (f.rt == 2) TREE_ROWS(64, 2); else TREE_ROWS(64, 1); }
