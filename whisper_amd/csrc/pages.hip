@@ -20,7 +20,7 @@ struct PageArgs {
     // append
     const char *rk, *rv;
     int64_t ks[4], vs[4];
-    int layer0;
+    int layer0, n_layers, per_group;   // per_group: layers a workgroup
     int es;                            // bytes an element
     int32_t* n_live;
 };
@@ -112,6 +112,43 @@ __global__ __launch_bounds__(128) void cache_fork_write_kernel(PageArgs a) {
         row[p] = p < keep ? from[2 + p] : -1;
     }
     if (threadIdx.x == 0) { c.d_lens[s] = len; c.d_held[s] = keep; }
+}
+
+// The same in one launch, by one workgroup that keeps what it read in LDS: lists of up to FK_ENTRIES x tables of up to FK_CELLS cells.
+constexpr int FK_ENTRIES = 512, FK_CELLS = 8192;
+__global__ __launch_bounds__(1024) void cache_fork_small_kernel(PageArgs a) {
+    __shared__ int cells[FK_CELLS], s_len[FK_ENTRIES], s_keep[FK_ENTRIES], s_held[FK_ENTRIES];
+    const wx_cache& c = a.c;
+    const int tid = threadIdx.x, MP = c.max_pages, n = a.n;
+    for (int i = tid; i < n; i += 1024) {
+        const int d = a.seqs[i], src = a.src[i];
+        bool ok = d >= 0 && d < c.max_seqs && src >= 0 && src < c.max_seqs;
+        for (int j = 0; j < i; ++j) ok &= a.seqs[j] != d;
+        const int len = ok ? c.d_lens[src] : -1;
+        s_len[i] = len;
+        s_keep[i] = len < 0 ? 0 : min((len + c.page_size - 1) / c.page_size, min(c.d_held[src], MP));
+        s_held[i] = len < 0 ? 0 : min(c.d_held[d], MP);
+        if (a.status) a.status[i] = len < 0 ? WX_ERR_INVALID : WX_OK;
+    }
+    __syncthreads();
+    for (int u = tid; u < n * MP; u += 1024) {
+        const int i = u / MP, q = u % MP;
+        int page = -1;
+        if (q < s_keep[i]) {
+            page = c.d_table[(int64_t)a.src[i] * MP + q];
+            if ((unsigned)page < (unsigned)c.n_pages) atomicAdd(&c.d_refs[page], 1);
+        }
+        cells[u] = page;
+    }
+    __syncthreads();
+    for (int u = tid; u < n * MP; u += 1024) {
+        const int i = u / MP, q = u % MP;
+        if (s_len[i] < 0 || q >= max(s_held[i], s_keep[i])) continue;
+        int32_t* cell = c.d_table + (int64_t)a.seqs[i] * MP + q;
+        if (q < s_held[i]) unref(c, *cell);
+        *cell = cells[u];
+    }
+    for (int i = tid; i < n; i += 1024) if (s_len[i] >= 0) { c.d_lens[a.seqs[i]] = s_len[i]; c.d_held[a.seqs[i]] = s_keep[i]; }
 }
 
 // inclusive sum over a workgroup of PG_NT threads; *total = the sum of all
@@ -239,24 +276,44 @@ __device__ __forceinline__ bool rows_private(const wx_cache& c, int s, int len, 
     return !__syncthreads_or(bad);
 }
 
-// ---- append: grid (entry, layer, keys / values) ----------------------------------------------------------------------------------
+// ---- append: grid (entry, group of AP_NODES nodes, group of layers) -------------------------------------------------------------------
+// The entry is checked and its places are looked up once for all layers of the group; a thread then takes its 16 bytes of keys and of
+// values through the layers, two layers' loads at a time.
+constexpr int AP_NODES = 4;
 __global__ __launch_bounds__(256) void cache_append_kernel(PageArgs a) {
+    __shared__ int64_t place[AP_NODES];
     const wx_cache& c = a.c;
-    const int i = blockIdx.x;
-    if (!entry_ok(a.seqs, i, c.max_seqs)) return;
-    const int s = a.seqs[i], len = c.d_lens[s];
+    const int i = blockIdx.x, j0 = blockIdx.y * AP_NODES;
     const int count = a.counts ? min(a.counts[i], a.n_nodes) : a.n_nodes;
+    if (j0 >= count || !entry_ok(a.seqs, i, c.max_seqs)) return;
+    const int s = a.seqs[i], len = c.d_lens[s];
     if (!rows_private(c, s, len, count)) return;
-    const int64_t row_b = (int64_t)c.head_dim * a.es, head_b = row_b * c.page_size, page_b = head_b * c.n_kv_head;
-    char* pool = (char*)(blockIdx.z ? c.d_v : c.d_k) + (int64_t)(a.layer0 + blockIdx.y) * c.n_pages * page_b;
-    const int64_t* st = blockIdx.z ? a.vs : a.ks;
-    const char* rows = (blockIdx.z ? a.rv : a.rk) + (blockIdx.y * st[0] + i * st[1]) * a.es;
-    const int per = (int)(row_b / 16), heads = c.n_kv_head;
-    const int32_t* row = c.d_table + (int64_t)s * c.max_pages;
-    for (int u = threadIdx.x; u < count * heads * per; u += 256) {
-        const int x = u % per, h = (u / per) % heads, j = u / (per * heads), t = len + j;
-        const int64_t to = row[t / c.page_size] * page_b + h * head_b + (t % c.page_size) * row_b + x * 16;
-        *reinterpret_cast<i32x4*>(pool + to) = *reinterpret_cast<const i32x4*>(rows + (j * st[2] + h * st[3]) * a.es + x * 16);
+    const int64_t row_b = (int64_t)c.head_dim * a.es, head_b = row_b * c.page_size, page_b = head_b * c.n_kv_head, layer_b = page_b * c.n_pages;
+    const int nodes = min(AP_NODES, count - j0), per = (int)(row_b / 16), heads = c.n_kv_head;
+    if (threadIdx.x < nodes) {
+        const int t = len + j0 + threadIdx.x;
+        place[threadIdx.x] = c.d_table[(int64_t)s * c.max_pages + t / c.page_size] * page_b + (t % c.page_size) * row_b;
+    }
+    __syncthreads();
+    const int l0 = blockIdx.z * a.per_group, l1 = min(a.n_layers, l0 + a.per_group);
+    for (int u = threadIdx.x; u < nodes * heads * per; u += 256) {
+        const int x = u % per, h = (u / per) % heads, j = u / (per * heads);
+        const char* k = a.rk + (l0 * a.ks[0] + i * a.ks[1] + (j0 + j) * a.ks[2] + h * a.ks[3]) * a.es + x * 16;
+        const char* v = a.rv + (l0 * a.vs[0] + i * a.vs[1] + (j0 + j) * a.vs[2] + h * a.vs[3]) * a.es + x * 16;
+        const int64_t to = (a.layer0 + l0) * layer_b + place[j] + h * head_b + x * 16;
+        char *kt = (char*)c.d_k + to, *vt = (char*)c.d_v + to;
+        const int64_t kstep = a.ks[0] * a.es, vstep = a.vs[0] * a.es;
+        int l = l0;
+        for (; l + 1 < l1; l += 2, k += 2 * kstep, v += 2 * vstep, kt += 2 * layer_b, vt += 2 * layer_b) {
+            const i32x4 k0 = *reinterpret_cast<const i32x4*>(k), k1 = *reinterpret_cast<const i32x4*>(k + kstep);
+            const i32x4 v0 = *reinterpret_cast<const i32x4*>(v), v1 = *reinterpret_cast<const i32x4*>(v + vstep);
+            *reinterpret_cast<i32x4*>(kt) = k0; *reinterpret_cast<i32x4*>(kt + layer_b) = k1;
+            *reinterpret_cast<i32x4*>(vt) = v0; *reinterpret_cast<i32x4*>(vt + layer_b) = v1;
+        }
+        if (l < l1) {
+            const i32x4 k0 = *reinterpret_cast<const i32x4*>(k), v0 = *reinterpret_cast<const i32x4*>(v);
+            *reinterpret_cast<i32x4*>(kt) = k0; *reinterpret_cast<i32x4*>(vt) = v0;
+        }
     }
 }
 
@@ -277,27 +334,50 @@ __device__ __forceinline__ bool commit_ok(const PageArgs& a, int i, int* taken) 
     if (last >= 0x40000000) return false;
     return rows_private(c, a.seqs[i], c.d_lens[a.seqs[i]], last + 1);
 }
-// grid (entry, layer, keys / values): a thread takes 16 bytes of a head's rows down the whole path.  path[k] >= k and ascends, so a
-// row that is overwritten was read before by the same thread; rows that stay (path[k] == k) are not touched.
+// grid (entry, group of layers): a thread takes 16 bytes of a head's rows of one layer, keys or values, down the whole path.  path[k] >= k
+// and ascends, so a row that is overwritten was read before by the same thread (eight rows are read before they are written); rows that
+// stay (path[k] == k) are not touched.  Where one group holds all layers, the workgroup sets the length itself.
+constexpr int CM_ROWS = 64;                                          // moves looked up at a time
 __global__ __launch_bounds__(256) void cache_commit_rows_kernel(PageArgs a) {
+    __shared__ int64_t from[CM_ROWS], to[CM_ROWS];
     const wx_cache& c = a.c;
     const int i = blockIdx.x;
     int taken;
-    if (!commit_ok(a, i, &taken)) return;
+    const bool ok = commit_ok(a, i, &taken);
+    const bool all = gridDim.y == 1;
+    if (all && threadIdx.x == 0 && a.status) a.status[i] = ok ? WX_OK : WX_ERR_INVALID;
+    if (!ok) return;
     const int s = a.seqs[i], len = c.d_lens[s];
     const int32_t* path = a.path + (int64_t)i * a.n_nodes;
     const int32_t* row = c.d_table + (int64_t)s * c.max_pages;
-    const int64_t row_b = (int64_t)c.head_dim * a.es, head_b = row_b * c.page_size, page_b = head_b * c.n_kv_head;
-    char* pool = (char*)(blockIdx.z ? c.d_v : c.d_k) + (int64_t)blockIdx.y * c.n_pages * page_b;
-    const int per = (int)(row_b / 16);
-    for (int u = threadIdx.x; u < c.n_kv_head * per; u += 256) {
-        char* col = pool + (u / per) * head_b + (u % per) * 16;
-        for (int k = 0; k < taken; ++k) {
-            if (path[k] == k) continue;
-            const int from = len + path[k], to = len + k;
-            *reinterpret_cast<i32x4*>(col + row[to / c.page_size] * page_b + (to % c.page_size) * row_b) =
-                *reinterpret_cast<const i32x4*>(col + row[from / c.page_size] * page_b + (from % c.page_size) * row_b);
+    const int64_t row_b = (int64_t)c.head_dim * a.es, head_b = row_b * c.page_size, page_b = head_b * c.n_kv_head, layer_b = page_b * c.n_pages;
+    const int per = (int)(row_b / 16), cols = c.n_kv_head * per, l0 = blockIdx.y * a.per_group, layers = min(c.n_layer, l0 + a.per_group) - l0;
+    int k0 = 0;
+    while (k0 < taken && path[k0] == k0) ++k0;                        // (uniform; the rows of a draft whose first branch was taken stay)
+    for (; k0 < taken; k0 += CM_ROWS) {
+        const int moves = min(CM_ROWS, taken - k0);
+        __syncthreads();
+        for (int k = threadIdx.x; k < moves; k += 256) {
+            const int f = len + path[k0 + k], t = len + k0 + k;
+            from[k] = row[f / c.page_size] * page_b + (f % c.page_size) * row_b;
+            to[k] = row[t / c.page_size] * page_b + (t % c.page_size) * row_b;
         }
+        __syncthreads();
+        for (int u = threadIdx.x; u < cols * layers * 2; u += 256) {
+            const int col = u % cols, w = u / cols;                  // w: layer, keys / values
+            char* pool = (char*)(w & 1 ? c.d_v : c.d_k) + (l0 + (w >> 1)) * layer_b + (col / per) * head_b + (col % per) * 16;
+            for (int k = 0; k < moves; k += 8) {
+                i32x4 x[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) x[q] = *reinterpret_cast<const i32x4*>(pool + from[min(k + q, moves - 1)]);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) if (k + q < moves) *reinterpret_cast<i32x4*>(pool + to[k + q]) = x[q];
+            }
+        }
+    }
+    if (all) {
+        __syncthreads();
+        if (threadIdx.x == 0) c.d_lens[s] = len + taken;
     }
 }
 __global__ __launch_bounds__(64) void cache_commit_len_kernel(PageArgs a) {
@@ -403,6 +483,10 @@ int wx_cache_fork(const wx_cache* c, const int32_t* d_dst, const int32_t* d_src,
     OnDevice on(c->device);
     PageArgs a = page_args(c, d_dst, n, d_status);
     a.src = d_src;
+    if (n <= FK_ENTRIES && (int64_t)n * c->max_pages <= FK_CELLS) {
+        hipLaunchKernelGGL(cache_fork_small_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
+        PG_DONE();
+    }
     hipLaunchKernelGGL(cache_fork_read_kernel, dim3(n), dim3(128), 0, (hipStream_t)stream, a);
     hipLaunchKernelGGL(cache_fork_write_kernel, dim3(n), dim3(128), 0, (hipStream_t)stream, a);
     PG_DONE();
@@ -435,8 +519,12 @@ int wx_cache_append(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_c
     }
     if (((uintptr_t)d_k | (uintptr_t)d_v) & 15) return set_error(WX_ERR_INVALID, "rows must be 16-byte aligned");
     OnDevice on(c->device);
-    a.counts = d_counts; a.n_nodes = n_nodes; a.layer0 = layer0; a.rk = (const char*)d_k; a.rv = (const char*)d_v;
-    hipLaunchKernelGGL(cache_append_kernel, dim3(n, n_layers, 2), dim3(256), 0, (hipStream_t)stream, a);
+    a.counts = d_counts; a.n_nodes = n_nodes; a.layer0 = layer0; a.n_layers = n_layers; a.rk = (const char*)d_k; a.rv = (const char*)d_v;
+    // as many layers a workgroup as leave 2048 workgroups (8 on every CU): the look-up is paid once for them
+    const int groups = (n_nodes + AP_NODES - 1) / AP_NODES;
+    const int64_t z = (2048 + (int64_t)n * groups - 1) / ((int64_t)n * groups);
+    a.per_group = (int)((n_layers + z - 1) / z);
+    hipLaunchKernelGGL(cache_append_kernel, dim3(n, groups, (n_layers + a.per_group - 1) / a.per_group), dim3(256), 0, (hipStream_t)stream, a);
     PG_DONE();
 }
 
@@ -449,8 +537,13 @@ int wx_cache_commit(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_p
     OnDevice on(c->device);
     PageArgs a = page_args(c, d_seqs, n, d_status);
     a.path = d_path; a.counts = d_counts; a.n_nodes = n_nodes;
-    hipLaunchKernelGGL(cache_commit_rows_kernel, dim3(n, c->n_layer, 2), dim3(256), 0, (hipStream_t)stream, a);
-    hipLaunchKernelGGL(cache_commit_len_kernel, dim3(n), dim3(64), 0, (hipStream_t)stream, a);
+    // one workgroup an entry where a token's rows of all layers are at most 32 KiB: no second launch for the lengths
+    const int64_t token_b = 2 * (int64_t)c->n_layer * c->n_kv_head * c->head_dim * a.es;
+    const int64_t y = token_b <= 32768 ? 1 : (1024 + n - 1) / n;
+    a.per_group = (int)((c->n_layer + y - 1) / y);
+    const int groups = (c->n_layer + a.per_group - 1) / a.per_group;
+    hipLaunchKernelGGL(cache_commit_rows_kernel, dim3(n, groups), dim3(256), 0, (hipStream_t)stream, a);
+    if (groups > 1) hipLaunchKernelGGL(cache_commit_len_kernel, dim3(n), dim3(64), 0, (hipStream_t)stream, a);
     PG_DONE();
 }
 

@@ -47,6 +47,15 @@ __device__ __forceinline__ int64_t tree_all(const wx_cache& c, const wx_tree_att
     return all;
 }
 
+struct TreeArgs { wx_cache c; wx_tree_attn a; TreePlan p; };
+// The arguments anew for every job: kept over the loop of jobs, they take the scalar registers and spill into vector registers.
+#define TREE_ARGS(ka) \
+    const __attribute__((address_space(4))) TreeArgs* ka##_p = (const __attribute__((address_space(4))) TreeArgs*)__builtin_amdgcn_kernarg_segment_ptr(); \
+    asm volatile("" : "+s"(ka##_p)); \
+    const wx_cache& c = ((const TreeArgs*)ka##_p)->c; \
+    const wx_tree_attn& a = ((const TreeArgs*)ka##_p)->a; \
+    const TreePlan& p = ((const TreeArgs*)ka##_p)->p
+
 // What a workgroup has to do now: sequence entry i, key / value head, block of rows, tiles [t0, t1) of the sequence's n_pre + tree_tiles.
 struct TreeJob {
     int ok;                  // 0: the rows are 0 (padding, no nodes), 1: attend, 2: refused (NaN), -1: nothing (any more)
@@ -365,7 +374,7 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // values (through the wave's own LDS, for the transposing read); the next tile's 16 loads a lane are issued as soon as the scores of
 // this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
 template <typename T, int D, int RT, bool ONE>
-__global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
+__global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
     typedef typename Elem<T>::Frag Frag;
     constexpr int E = 16 / sizeof(T), KT = 8192 / (D * (int)sizeof(T)), NS = KT / 16, KS = D / (4 * E), CPR = D / E, NV = KT * CPR / 64;
     constexpr int VROW = D * (int)sizeof(T) + Elem<T>::PAD, VBYTES = KT * VROW, OROW = 68;
@@ -377,7 +386,9 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c,
     __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, r = lane & 15;
     TreeJob j;
-    for (bool first = true; tree_next<KT, ONE>(c, a, p, &s_job, j, first); first = false) {
+    for (bool first = true;; first = false) {
+    TREE_ARGS(ka);
+    if (!tree_next<KT, ONE>(c, a, p, &s_job, j, first)) break;
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * RT * 16;
     if (wid == 0 && j.ok == 1) {
         bool wrong;
@@ -587,24 +598,23 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(wx_cache c,
 
 // ---- many rows (bf16): every wave has rows of its own, the workgroup shares the tiles of keys and values ------------------------------
 // Eight waves, RT x 16 rows each (two waves on every SIMD of a CU).  Tiles of 64 keys go from HBM to LDS without registers
-// (global_load_lds) into a ring of four, two to three tiles ahead; a wave-instruction writes 1 KiB of rows in a line, so the swizzle
+// (global_load_lds) into a ring of four, three tiles before their use; a wave-instruction writes 1 KiB of rows in a line, so the swizzle
 // that the fragment reads need (16-byte chunk x of a row in slot x ^ (row mod chunks)) is applied to its lanes' source addresses.
 // The softmax of a tile takes the vector pipe about as long as its two products take the matrix pipe.  So waves 4-7 run half a tile
 // behind waves 0-3, a barrier each half: while one wave of a SIMD does PV(t - 1) and QK(t), the other does the softmax of its tile.
 //
-// 16 bytes a lane from global memory to LDS address `to` + 16 x lane (alike on the wave).  Written out because the compiler, which knows
+// 16 bytes a lane from global memory (`from`, alike on the wave, + lane_off) to LDS address `to` + 16 x lane.  Written out because the compiler, which knows
 // of the builtin's LDS write, waits for ALL loads before every transposing LDS read, whatever they write; the waits are the kernel's own.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"                            // m0 is named as changed on purpose
-__device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(to) : "m0", "memory");
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t lane_off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(lane_off), "s"(from), "s"(to) : "m0", "memory");
 }
 #pragma clang diagnostic pop
-typedef const __attribute__((address_space(4))) int32_t const_i32;        // page numbers that are alike on a wave, by scalar loads
 constexpr int TRW = 8;                                                    // waves
 
 template <int D, int RT, bool ONE>
-__global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
+__global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeArgs) {
     typedef bf16 T;
     typedef bf16x8 Frag;
     constexpr int KT = 64, NS = 4, KS = D / 32, CPR = D / 8, ROWB = D * 2, HALF = KT * ROWB, RING = 4;
@@ -616,8 +626,10 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(wx_cac
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
     const bool late = wid >= TRW / 2;
     TreeJob j;
-    for (bool first = true; tree_next<KT, ONE>(c, a, p, &s_job, j, first); first = false) {
-    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * TRW * 16 * RT + wid * 16 * RT;
+    for (bool first = true;; first = false) {
+    TREE_ARGS(ka);
+    if (!tree_next<KT, ONE>(c, a, p, &s_job, j, first)) break;
+    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, part_row0 = ((wid & 3) * 2 + (wid >> 2)) * 16 * RT, row0 = j.rb * TRW * 16 * RT + part_row0;
     if (wid == 0 && j.ok == 1) {
         bool wrong;
         const uint64_t m = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
@@ -651,27 +663,50 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(wx_cac
         const T* Vp = reinterpret_cast<const T*>(c.d_v) + head_off;
         const int t0 = __builtin_amdgcn_readfirstlane(j.t0), n_tiles = __builtin_amdgcn_readfirstlane(min(j.t1, j.n_pre)) - t0;
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
-        const const_i32* ctable = (const const_i32*)(uintptr_t)table;
-        // this wave's rows of tile t (all on one page: RPW divides 16) -> its place in the ring
-        auto page_of = [&](int t) { return ctable[min((t0 + t) * KT + wid * RPW, len - 1) >> p.shift]; };
-        auto issue = [&](int t, int page) {
-            const int64_t base = (int64_t)page * page_e;
-            const uint32_t to = lds0 + (t & (RING - 1)) * 2 * HALF + wid * RPW * ROWB;
+        // this wave's rows of a tile are on one page (RPW divides 16): the pages of 64 tiles, one a lane
+        int pages = 0;
+        auto page_of = [&](int t) {
+            if ((t & 63) == 0) {
+                pages = table[min((t0 + min(t + lane, n_tiles - 1)) * KT + wid * RPW, len - 1) >> p.shift];
+                __builtin_amdgcn_s_waitcnt(0x0f70);                                // vmcnt(0): here, not by the compiler in every tile
+            }
+            return __builtin_amdgcn_readlane(pages, t & 63);
+        };
+        // no vector instructions but in the last tile: everything but the lane's place in the rows is alike on the wave
+        uint32_t lane_off[NL];
 #pragma unroll
-            for (int x = 0; x < NL; ++x) {
-                const int row = wid * RPW + x * RPL + lane / CPR, at = min((t0 + t) * KT + row, len - 1);
-                const int64_t off = base + (int64_t)(at & (c.page_size - 1)) * D + ((lane % CPR) ^ (row & (CPR - 1))) * 8;
-                load_to_lds(Kp + off, to + x * 1024);
-                load_to_lds(Vp + off, to + HALF + x * 1024);
+        for (int x = 0; x < NL; ++x) {
+            const int row = x * RPL + lane / CPR;
+            lane_off[x] = row * ROWB + ((lane % CPR) ^ ((wid * RPW + row) & (CPR - 1))) * 16;
+        }
+        auto issue = [&](const T* pool, int half, int t, int page) {
+            const int at = (t0 + t) * KT + wid * RPW, live = len - at;               // rows of this wave that are tokens
+            const char* from = reinterpret_cast<const char*>(pool) + ((int64_t)page * page_e + (int64_t)(at & (c.page_size - 1)) * D) * 2;
+            const uint32_t to = lds0 + (t & (RING - 1)) * 2 * HALF + half + wid * RPW * ROWB;
+            if (live >= RPW) {
+#pragma unroll
+                for (int x = 0; x < NL; ++x) load_to_lds(from, lane_off[x], to + x * 1024);
+            } else {                                                                // rows past the last token read it instead
+                if (live <= 0) from = reinterpret_cast<const char*>(pool) + ((int64_t)page * page_e + (int64_t)((len - 1) & (c.page_size - 1)) * D) * 2;
+                const int last = max(live, 1) - 1;
+#pragma unroll
+                for (int x = 0; x < NL; ++x) {
+                    const int row = x * RPL + lane / CPR;
+                    load_to_lds(from, lane_off[x] - (row - min(row, last)) * ROWB, to + x * 1024);
+                }
             }
         };
-        // this wave's loads up to tile t are done (tile t + 1's, where there is one, may go on); rows past the last token count as 0 values
+        // Before QK(t) and PV(t - 1): this wave's loads of keys t and values t - 1 are done.  Issued behind them: keys t + 1, values t and, but by
+        // the late waves, who wait half a tile before they issue, keys t + 2, values t + 1; at the end there are fewer, and all are waited for.
         auto landed = [&](int t) {
-            if (t + 1 < n_tiles) {
+            if (t + 2 < n_tiles && (!late || t == 0)) {
+                if constexpr (NL == 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            } else if (t + 2 < n_tiles) {
                 if constexpr (NL == 2) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
                 else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
-            } else {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (t == n_tiles - 1) {                                                // the last tile's values are here too: rows past the last token count as 0
                 const int live = len - (t0 + t) * KT;
                 if (live < KT) {
                     char* vb = lds + (t & (RING - 1)) * 2 * HALF + HALF;
@@ -688,21 +723,23 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(wx_cac
         // fragments of the next 16 keys (of the next 16 columns) are read while the matrix pipe works on these: the order is pinned, or the
         // compiler reads each right before its use and waits for LDS every time
         auto scores = [&](const char* kb, f32x4 (&s)[NS][RT]) {
-            Frag kf[2][KS];
+            constexpr int AHEAD = 2;
+            Frag kf[AHEAD + 1][KS];
             auto read = [&](int k) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kf[k & 1][ks] = *reinterpret_cast<const Frag*>(kb + (k * 16 + r) * ROWB + ((ks * 64) ^ kx));
+                for (int ks = 0; ks < KS; ++ks) kf[k % (AHEAD + 1)][ks] = *reinterpret_cast<const Frag*>(kb + (k * 16 + r) * ROWB + ((ks * 64) ^ kx));
                 __builtin_amdgcn_sched_barrier(0);
             };
-            read(0);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) read(k);
 #pragma unroll
             for (int k = 0; k < NS; ++k) {
-                if (k + 1 < NS) read(k + 1);
+                if (k + AHEAD < NS) read(k + AHEAD);
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
                     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) x = Elem<T>::qk(kf[k & 1][ks], qf[t][ks], x);
+                    for (int ks = 0; ks < KS; ++ks) x = Elem<T>::qk(kf[k % (AHEAD + 1)][ks], qf[t][ks], x);
                     s[k][t] = x;
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -742,42 +779,62 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(wx_cac
             }
         };
         Frag pf[RT][2];
+        const int count = __builtin_amdgcn_readfirstlane(j.count);
         if (n_tiles > 0) {
             __builtin_amdgcn_s_waitcnt(0);                                          // the counts below are of tiles' loads only (the builtin, so
             __builtin_amdgcn_sched_barrier(0);                                      // that the compiler does not wait for the queries in the loop)
-            issue(0, page_of(0));
-            if (n_tiles > 1) issue(1, page_of(1));
-            int page = page_of(min(2, n_tiles - 1));
+            const int page0 = page_of(0), page1 = page_of(1);
+            int page_v = page_of(2), page_k = page_of(3);                           // of tiles past the end: the last one's, not used
+            issue(Kp, 0, 0, page0);
+            if (n_tiles > 1) issue(Kp, 0, 1, page1);
+            issue(Vp, HALF, 0, page0);
+            if (n_tiles > 2) issue(Kp, 0, 2, page_v);
+            if (n_tiles > 1) issue(Vp, HALF, 1, page1);
             landed(0);
             barrier();
             if (late) barrier();
-            for (int t = 0; t < n_tiles; ++t) {
-                // the slot of tile t + 2 held tile t - 2, whose values the late waves read last, a barrier ago
-                if (t + 2 < n_tiles) { issue(t + 2, page); page = page_of(min(t + 3, n_tiles - 1)); }
-                __builtin_amdgcn_s_setprio(1);
-                if (t > 0) add(lds + ((t - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
-                f32x4 s[NS][RT];
-                scores(lds + (t & (RING - 1)) * 2 * HALF, s);
-                __builtin_amdgcn_s_setprio(0);
-                if (late && t + 1 < n_tiles) landed(t + 1);
-                barrier();
-                const int live = len - (t0 + t) * KT;
-                if (live < KT) {
-                    asm volatile("");                                               // keep it a branch: as selects it costs every tile
+            // Keys t + 3 take the place of keys t - 1, values t + 2 of values t - 2: the late waves read both last, two barriers ago for the
+            // early waves, one for themselves.  Issued with the softmax and not before the products, which are the longer half.
+            auto more = [&](int t) {
+                if (t + 3 < n_tiles) issue(Kp, 0, t + 3, page_k);
+                if (t + 2 < n_tiles) issue(Vp, HALF, t + 2, page_v);
+                page_v = page_k;
+                if (t + 4 < n_tiles) page_k = page_of(t + 4);
+            };
+            if (row0 < count * G) {
+                for (int t = 0; t < n_tiles; ++t) {
+                    if (t > 0) add(lds + ((t - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
+                    f32x4 s[NS][RT];
+                    scores(lds + (t & (RING - 1)) * 2 * HALF, s);
+                    if (late && t + 1 < n_tiles) landed(t + 1);
+                    barrier();
+                    more(t);
+                    const int live = len - (t0 + t) * KT;
+                    if (live < KT) {
+                        asm volatile("");                                           // keep it a branch: as selects it costs every tile
 #pragma unroll
-                    for (int k = 0; k < NS; ++k)
+                        for (int k = 0; k < NS; ++k)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            if (16 * k + 4 * g + x >= live)
+                            for (int x = 0; x < 4; ++x)
+                                if (16 * k + 4 * g + x >= live)
 #pragma unroll
-                                for (int q = 0; q < RT; ++q) s[k][q][x] = -INFINITY;
+                                    for (int q = 0; q < RT; ++q) s[k][q][x] = -INFINITY;
+                    }
+                    st.template softmax<NS>(s, cc);
+                    pack(s, pf);
+                    if (!late && t + 1 < n_tiles) landed(t + 1);
+                    barrier();
                 }
-                st.template softmax<NS>(s, cc);
-                pack(s, pf);
-                if (!late && t + 1 < n_tiles) landed(t + 1);
-                barrier();
+                add(lds + ((n_tiles - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
+            } else {                                                               // a wave of nodes that are not there only brings its rows
+                for (int t = 0; t < n_tiles; ++t) {
+                    if (late && t + 1 < n_tiles) landed(t + 1);
+                    barrier();
+                    more(t);
+                    if (!late && t + 1 < n_tiles) landed(t + 1);
+                    barrier();
+                }
             }
-            add(lds + ((n_tiles - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
             if (!late) barrier();
             __syncthreads();
         }
@@ -837,7 +894,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(wx_cac
             for (int d = 0; d < D / 16; ++d)
                 store4<T>(out + 16 * d + 4 * g, kind == 1 ? st.o[d][t] * f : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
         } else {
-            float* to = part + (int64_t)(wid * RT * 16 + t * 16 + r) * (D + 2);
+            float* to = part + (int64_t)(part_row0 + t * 16 + r) * (D + 2);
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
                 *reinterpret_cast<f32x2*>(to + 16 * d + 4 * g) = f32x2{st.o[d][t][0], st.o[d][t][1]};
@@ -890,15 +947,31 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
     const int node = row / G;
     const int64_t step = (int64_t)c.n_kv_head * p.row_blocks * p.rows * (D + 2);
     const float* part = p.part + ((((int64_t)first * c.n_kv_head + kh) * p.row_blocks + row / p.rows) * p.rows + row % p.rows) * (D + 2);
+    // four pieces' loads at a time, one running maximum (a launch of this size is bound by the loads' latency)
     float M = -INFINITY, L = 0.f;
-    for (int q = 0; q < pieces; ++q) M = fmaxf(M, part[q * step + D]);
     f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int q = 0; q < pieces; ++q) {
-        const float* from = part + q * step;
-        const float m = from[D], f = m == M ? 1.f : __builtin_amdgcn_exp2f((m - M) * cc);
-        L = fmaf(from[D + 1], f, L);
-        const f32x2 lo = *reinterpret_cast<const f32x2*>(from + x), hi = *reinterpret_cast<const f32x2*>(from + x + 2);
-        v += f32x4{lo[0], lo[1], hi[0], hi[1]} * f;
+    for (int q0 = 0; q0 < pieces; q0 += 4) {
+        float m[4], l[4];
+        f32x2 lo[4], hi[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float* from = part + min(q0 + q, pieces - 1) * step;
+            m[q] = from[D]; l[q] = from[D + 1];
+            lo[q] = *reinterpret_cast<const f32x2*>(from + x); hi[q] = *reinterpret_cast<const f32x2*>(from + x + 2);
+        }
+        float mn = M;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mn = fmaxf(mn, m[q]);
+        const float old = M == mn ? 1.f : __builtin_amdgcn_exp2f((M - mn) * cc);
+        M = mn;
+        L *= old; v *= old;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (q0 + q < pieces) {
+                const float f = m[q] == mn ? 1.f : __builtin_amdgcn_exp2f((m[q] - mn) * cc);
+                L = fmaf(l[q], f, L);
+                v += f32x4{lo[q][0], lo[q][1], hi[q][0], hi[q][1]} * f;
+            }
     }
     T* out = reinterpret_cast<T*>(a.d_out) + i * a.o_seq + node * a.o_node + (kh * G + row % G) * a.o_head + x;
     const int kind = seq == -1 || node >= count ? 0 : s_wrong[node] ? 2 : 1;
@@ -915,7 +988,7 @@ static hipError_t launch_rows(dim3 grid, int lds, hipStream_t st, const wx_cache
         if (e != hipSuccess) return e;
         asked.fetch_or(bit, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL((tree_attention_rows_kernel<D, RT, ONE>), grid, dim3(64 * TRW), lds, st, c, a, p);
+    hipLaunchKernelGGL((tree_attention_rows_kernel<D, RT, ONE>), grid, dim3(64 * TRW), lds, st, TreeArgs{c, a, p});
     return hipSuccess;
 }
 
@@ -956,34 +1029,81 @@ static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {
 
 // ---- verification ---------------------------------------------------------------------------------------------------------------------
 struct Best { float m, s; int i; };       // largest logit, sum of exp(logit - m), its lowest id
-__device__ __forceinline__ void best_add(Best& b, float v, int i) {
-    if (!(v > -INFINITY)) return;                                     // masked, or NaN
-    if (v > b.m) { b.s = b.s * __expf(b.m - v) + 1.f; b.m = v; b.i = i; }
-    else if (v == b.m) { b.s += 1.f; b.i = min(b.i, i); }             // also where both are +infinity
-    else b.s += __expf(v - b.m);
-}
 __device__ __forceinline__ Best best_merge(Best a, Best b) {
     if (a.m == b.m) return Best{a.m, a.s + b.s, min(a.i, b.i)};
     if (b.m > a.m) { const Best t = a; a = b; b = t; }
-    a.s += b.s * __expf(b.m - a.m);                                   // b.m may be -infinity: + 0
+    a.s += b.s * __builtin_amdgcn_exp2f((b.m - a.m) * TR_LOG2E);     // b.m may be -infinity: + 0
     return a;
 }
-constexpr int VF_NT = 256;
+// N values of ids i .. i + N - 1 (masked ones are -infinity).  The maximum of all of them comes first, so that the running sum is rescaled
+// once for N ids, and seldom; v - m is rounded before it is scaled, or the rounding of m log2 e would shift every term.
+template <int N>
+__device__ __forceinline__ void best_add(Best& b, float (&v)[N], int i) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < N; ++j) { v[j] = fmaxf(v[j], -INFINITY); top = fmaxf(top, v[j]); }        // NaN counts as masked
+    if (top > b.m) {
+        b.s *= __builtin_amdgcn_exp2f((b.m - top) * TR_LOG2E);
+        b.m = top;
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j) if (v[j] == top) b.i = i + j;
+    }
+    if (b.m == INFINITY) {                                            // infinite logits share the probability
+#pragma unroll
+        for (int j = 0; j < N; ++j) b.s += v[j] == INFINITY ? 1.f : 0.f;
+    } else if (b.m > -INFINITY) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) b.s += __builtin_amdgcn_exp2f((v[j] - b.m) * TR_LOG2E);
+    }
+}
+constexpr int VF_NT = 256, VF_U = 4;       // VF_U 16-byte loads a thread are in flight
 
-// one workgroup a (part of the vocabulary, node, sequence): one pass over the logits
+// One workgroup a (part of the vocabulary, node, sequence): one pass over the logits, 16 bytes a lane.  Bound by their stream.
 template <typename T>
 __global__ __launch_bounds__(VF_NT) void tree_verify_scan_kernel(wx_tree_check a, int parts) {
+    constexpr int E = 16 / sizeof(T);
     __shared__ Best sh[VF_NT / 64];
     const int part = blockIdx.x, node = blockIdx.y, i = blockIdx.z, tid = threadIdx.x;
     const int count = a.d_counts ? a.d_counts[i] : a.n_nodes;
     if (node >= count) return;
-    const int per = (a.n_vocab + parts - 1) / parts, lo = part * per, hi = min(a.n_vocab, lo + per);
     const T* row = reinterpret_cast<const T*>(a.d_logits) + i * a.l_seq + node * a.l_node;
-    Best b{-INFINITY, 0.f, 0x7fffffff};
-    for (int x = lo + tid; x < hi; x += VF_NT) {
-        if (a.d_suppress && a.d_suppress[x]) continue;
-        best_add(b, (float)row[x], x);
+    // aligned 16-byte units of the row; the ids before the first and after the last (fewer than 16) go one by one, with part 0
+    const int head = min(a.n_vocab, (int)(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(T))), units = (a.n_vocab - head) / E;
+    const int per = (units + parts - 1) / parts, lo = part * per, hi = min(units, lo + per);
+    const uint8_t* sup = a.d_suppress;
+    Best h{-INFINITY, 0.f, 0x7fffffff}, b = h;
+    if (part == 0 && tid < a.n_vocab - units * E) {
+        const int x = tid < head ? tid : units * E + tid;
+        float v[1] = {sup && sup[x] ? -INFINITY : (float)row[x]};
+        best_add<1>(h, v, x);
     }
+    typedef __attribute__((ext_vector_type(E))) T Unit;
+    for (int u0 = lo + tid; u0 < hi; u0 += VF_NT * VF_U) {
+        Unit x[VF_U];
+        uint32_t m[VF_U][E / 4];
+#pragma unroll
+        for (int k = 0; k < VF_U; ++k) {
+            const int u = min(u0 + k * VF_NT, units - 1);
+            x[k] = __builtin_nontemporal_load(reinterpret_cast<const Unit*>(row + head) + u);
+            if (sup) __builtin_memcpy(m[k], sup + head + u * E, E);
+            else __builtin_memset(m[k], 0, E);
+        }
+#pragma unroll
+        for (int k = 0; k < VF_U; ++k) {
+            if (u0 + k * VF_NT >= hi) break;
+            float v[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = (float)x[k][j];
+            uint32_t any = m[k][0];
+            if constexpr (E == 8) any |= m[k][1];
+            if (any) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) if ((m[k][j / 4] >> (8 * (j % 4))) & 0xff) v[j] = -INFINITY;
+            }
+            best_add<E>(b, v, head + (u0 + k * VF_NT) * E);
+        }
+    }
+    b = best_merge(b, h);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) {
         Best o;
@@ -1086,8 +1206,8 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
     if (jobs > 0x7fffffff) return set_error(WX_ERR_INVALID, "too many pieces: larger split_tokens, or fewer sequences");
     const dim3 grid((unsigned)jobs), block(256);
     const bool f32 = c->precision == WX_PREC_F32, wide = c->head_dim == 128;
-#define TREE_KEYS(T, D, RT) do { if (p.single) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, true>), grid, block, 0, st, *c, *a, p); \
-                                 else hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, false>), grid, block, 0, st, *c, *a, p); } while (0)
+#define TREE_KEYS(T, D, RT) do { if (p.single) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, true>), grid, block, 0, st, TreeArgs{*c, *a, p}); \
+                                 else hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, false>), grid, block, 0, st, TreeArgs{*c, *a, p}); } while (0)
 #define TREE_ROWS(D, RT) do { const int lds = 4 * 2 * 64 * D * 2; \
                               const hipError_t le = p.single ? launch_rows<D, RT, true>(grid, lds, st, *c, *a, p) : launch_rows<D, RT, false>(grid, lds, st, *c, *a, p); \
                               if (le != hipSuccess) return set_error(WX_ERR_HIP, hipGetErrorString(le)); } while (0)

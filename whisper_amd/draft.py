@@ -34,13 +34,13 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: Optional[to
         if not torch.is_tensor(t) or t.dtype != dtype or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
             raise ValueError(f"{what} must be a contiguous {dtype} tensor {list(shape)} on {dev}")
     lib = _lib.load()
-    i32 = torch.empty((2, n, nodes), dtype=torch.int32, device=dev)
-    ends = torch.empty((2, n), dtype=torch.int32, device=dev)
+    i32 = dict(dtype=torch.int32, device=dev)
+    pick, path, accept, follow = torch.empty((n, nodes), **i32), torch.empty((n, nodes), **i32), torch.empty(n, **i32), torch.empty(n, **i32)
     logprob = torch.empty((n, nodes), dtype=torch.float32, device=dev)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    a = _lib.WxTreeCheck(n, nodes, vocab, _PRECISION[logits.dtype], dev.index, logits.data_ptr(), logits.stride(0), logits.stride(1), ptr(tokens),
-                         ptr(parents), ptr(counts), ptr(suppress), i32.data_ptr(), logprob.data_ptr(), i32[1].data_ptr(), ends.data_ptr(),
-                         ends[1].data_ptr())
+    a = _lib.WxTreeCheck(n, nodes, vocab, _PRECISION[logits.dtype], dev.index, logits.data_ptr(), logits.stride(0), logits.stride(1), tokens.data_ptr(),
+                         None if parents is None else parents.data_ptr(), None if counts is None else counts.data_ptr(),
+                         None if suppress is None else suppress.data_ptr(), pick.data_ptr(), logprob.data_ptr(), path.data_ptr(), accept.data_ptr(),
+                         follow.data_ptr())
     ref = ctypes.byref(a)
     need = lib.wx_tree_verify_work_bytes(ref)
     if need < 0:
@@ -48,4 +48,4 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: Optional[to
     work = torch.empty(need, dtype=torch.uint8, device=dev)
     a.d_work, a.work_bytes = work.data_ptr(), need
     _check(lib.wx_tree_verify(ref, _raw_stream(dev.index)), "wx_tree_verify")
-    return {"pick": i32[0], "logprob": logprob, "path": i32[1], "n_accept": ends[0], "next": ends[1]}
+    return {"pick": pick, "logprob": logprob, "path": path, "n_accept": accept, "next": follow}
