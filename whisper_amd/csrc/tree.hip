@@ -80,10 +80,10 @@ __device__ __forceinline__ void tree_fill(const wx_cache& c, const wx_tree_attn&
 }
 
 // The first job of a workgroup (first = true) or the next of its share; *sh is the same on every thread afterwards.
-template <int KT, bool ONE>
+template <int KT>
 __device__ __forceinline__ bool tree_next(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob* sh, TreeJob& j, bool first) {
     const int tid = threadIdx.x, lane = tid & 63;
-    if (!first && (ONE || p.per)) return false;
+    if (!first && p.per) return false;
     __syncthreads();                                               // the job before is done with *sh and the other shared arrays
     if (tid < 64) {
         TreeJob t;
@@ -93,7 +93,7 @@ __device__ __forceinline__ bool tree_next(const wx_cache& c, const wx_tree_attn&
             t.kh = w % c.n_kv_head; t.rb = y % p.row_blocks; t.w = w / c.n_kv_head; t.whole = 1; t.piece = 0; t.i = t.w; t.takers = 0;
             t.all = t.start = t.x0 = t.x1 = 0;
             t.ok = t.w < p.slots ? 1 : -1;
-            if (t.ok == 1 && !ONE) {
+            if (t.ok == 1) {
                 if (p.per) {                                       // piece number t.w, counted through the sequences
                     int before = 0;
                     t.ok = -1;
@@ -141,8 +141,7 @@ __device__ __forceinline__ bool tree_next(const wx_cache& c, const wx_tree_attn&
         if (t.ok == 1) {
             tree_fill(c, a, p, KT, t);
             const int tiles = t.n_pre + p.tree_tiles;
-            if (ONE) { t.t0 = 0; t.t1 = tiles; }
-            else if (p.per) { t.t0 = (int)t.x0; t.t1 = (int)min(t.x1, (int64_t)tiles); }
+            if (p.per) { t.t0 = (int)t.x0; t.t1 = (int)min(t.x1, (int64_t)tiles); }
             else {
                 t.t0 = (int)max((int64_t)0, t.x0 - t.start); t.t1 = (int)min((int64_t)tiles, t.x1 - t.start);
                 t.whole = tree_taker(t.start, t.all, t.takers) == tree_taker(t.start + tiles - 1, t.all, t.takers);
@@ -155,21 +154,36 @@ __device__ __forceinline__ bool tree_next(const wx_cache& c, const wx_tree_attn&
     __syncthreads();
     j = *sh;
     if (j.ok < 0) return false;
-    int bad = 0;
-    if (j.ok == 1) {
-        // the pages of this piece's tiles (of the draft's rows too, which have to be this slot's alone where they are written)
-        const int32_t* row = c.d_table + (int64_t)j.seq * c.max_pages;
-        const int upto = j.t1 > j.n_pre ? j.len + j.count : min(j.len, j.t1 * KT);
-        const int own = a.d_kn && j.last ? j.len >> p.shift : 0x7fffffff;
-        for (int q = (min(j.t0 * KT, j.len) >> p.shift) + tid; q << p.shift < upto; q += blockDim.x) {
-            const int page = row[q];
-            if ((unsigned)page >= (unsigned)c.n_pages || (q >= own && c.d_refs[page] != 1)) bad = 1;
-        }
-        if (a.d_kn) for (int k = tid; k < j.i; k += blockDim.x) bad |= a.d_seqs[k] == j.seq;
-    }
-    if (__syncthreads_or(bad)) { j.ok = 2; if (tid == 0) sh->ok = 2; }             // (read again behind the caller's next barrier)
     return true;
 }
+// The one job of a workgroup that does one whole sequence: no search, and nothing waits for another wave.
+template <int KT>
+__device__ __forceinline__ bool tree_whole(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob& t) {
+    const int lin = blockIdx.x, y = lin / 8, w = (y / p.row_blocks) * 8 + lin % 8;     // (as tree_next)
+    t.kh = w % c.n_kv_head; t.rb = y % p.row_blocks; t.i = t.w = w / c.n_kv_head; t.whole = 1; t.piece = 0; t.takers = 0; t.last = 1;
+    t.all = t.start = t.x0 = t.x1 = 0;
+    if (t.w >= p.slots) return false;
+    tree_fill(c, a, p, KT, t);
+    t.t0 = 0; t.t1 = t.n_pre + p.tree_tiles;
+    return true;
+}
+// A job's second look, by all threads of the workgroup, each with its share of it: whether a page of the piece's tiles is none of the
+// pool's, a page of the draft's rows is not this slot's alone although they are to be written, or an appending call names the slot
+// before.  What comes of it is needed at the end only (nothing is written before, and page_ok() keeps the reads inside the pool), so that
+// its loads overlap the work.
+__device__ __forceinline__ int tree_bad(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, int kt) {
+    int bad = 0;
+    const int32_t* row = c.d_table + (int64_t)j.seq * c.max_pages;
+    const int upto = j.t1 > j.n_pre ? j.len + j.count : min(j.len, j.t1 * kt);
+    const int own = a.d_kn && j.last ? j.len >> p.shift : 0x7fffffff;
+    for (int q = (min(j.t0 * kt, j.len) >> p.shift) + threadIdx.x; q << p.shift < upto; q += blockDim.x) {
+        const int page = row[q];
+        if ((unsigned)page >= (unsigned)c.n_pages || (q >= own && c.d_refs[page] != 1)) bad = 1;
+    }
+    if (a.d_kn) for (int k = threadIdx.x; k < j.i; k += blockDim.x) bad |= a.d_seqs[k] == j.seq;
+    return bad;
+}
+__device__ __forceinline__ int page_ok(const wx_cache& c, int page) { return (unsigned)page < (unsigned)c.n_pages ? page : 0; }
 
 // bit j of the result, on lane i of a wave: node j is node i or one of its ancestors.  *bad: node i hangs on a parent out of range.
 // Doubling: after k steps a lane knows 2^k ancestors and jumps that far.
@@ -318,7 +332,7 @@ __device__ __forceinline__ const T* node_row(const wx_cache& c, const wx_tree_at
         return keys ? reinterpret_cast<const T*>(a.d_kn) + j.i * a.kn_seq + node * a.kn_node + j.kh * a.kn_head
                     : reinterpret_cast<const T*>(a.d_vn) + j.i * a.vn_seq + node * a.vn_node + j.kh * a.vn_head;
     const int t = j.len + node;
-    return reinterpret_cast<const T*>(keys ? c.d_k : c.d_v) + head_off + table[t >> p.shift] * page_e + (int64_t)(t & (c.page_size - 1)) * D;
+    return reinterpret_cast<const T*>(keys ? c.d_k : c.d_v) + head_off + page_ok(c, table[t >> p.shift]) * page_e + (int64_t)(t & (c.page_size - 1)) * D;
 }
 
 // The rare end of a tile of drafted rows whose values hold infinities or NaN: the matrix product ran on 0 in their place (0 x NaN would
@@ -381,35 +395,27 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
     constexpr int LDS = 4 * VBYTES > 4 * RT * 16 * OROW * 4 ? 4 * VBYTES : 4 * RT * 16 * OROW * 4;
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     __shared__ TreeJob s_job;
-    __shared__ uint64_t s_mask[64];
     __shared__ int s_wrong[64];
     __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, r = lane & 15;
     TreeJob j;
     for (bool first = true;; first = false) {
     TREE_ARGS(ka);
-    if (!tree_next<KT, ONE>(c, a, p, &s_job, j, first)) break;
+    if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j)) break; }
+    else if (!tree_next<KT>(c, a, p, &s_job, j, first)) break;
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * RT * 16;
-    if (wid == 0 && j.ok == 1) {
-        bool wrong;
-        const uint64_t m = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
-        s_mask[lane] = m; s_wrong[lane] = wrong;
-    }
-    __syncthreads();
+    int bad = 0;
     const int32_t* table = c.d_table + (int64_t)j.seq * c.max_pages;
     const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)j.kh * c.page_size * D;
     RowState<D, RT> st;
     st.init();
     if (j.ok == 1) {
-        if (a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
         Frag qf[RT][KS];
-        uint64_t mask[RT];
         const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f, cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const int row = min(row0 + t * 16 + r, rows - 1), node = row / G;
             const T* q = reinterpret_cast<const T*>(a.d_q) + j.i * a.q_seq + node * a.q_node + (j.kh * G + row % G) * a.q_head;
-            mask[t] = s_mask[node];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 qf[t][ks] = *reinterpret_cast<const Frag*>(q + (ks * 4 + g) * E);
@@ -424,7 +430,7 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
         char* vb = lds + wid * VBYTES;
         Frag kf[NS][KS], vr[NV];
         // a tile's pages: one for each 16 tokens, on lanes 0 .. NS-1
-        auto load_ids = [&](int t) { return table[min(t * KT + 16 * min(lane, NS - 1), j.len - 1) >> p.shift]; };
+        auto load_ids = [&](int t) { return page_ok(c, table[min(t * KT + 16 * min(lane, NS - 1), j.len - 1) >> p.shift]); };
         auto load_pre = [&](int t, int ids) {
             const int last = j.len - 1 - t * KT;                                  // >= 0
 #pragma unroll
@@ -478,10 +484,12 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
         };
         const int end = min(j.t1, j.n_pre);
         int t = j.t0 + wid;
-        if (t < end) {
+        if (t >= end) bad = tree_bad(c, a, p, j, KT);
+        else {
             int ids = load_ids(t);
             load_pre(t, ids);
             ids = load_ids(min(t + 4, j.n_pre - 1));
+            bad = tree_bad(c, a, p, j, KT);
             for (; t < end; t += 4) {
                 f32x4 s[NS][RT];
                 const int live = j.len - t * KT;
@@ -506,7 +514,16 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
                 __builtin_amdgcn_wave_barrier();
             }
         }
-        // the drafted rows' tiles go on in the same rotation of waves
+        // the drafted rows' tiles go on in the same rotation of waves; every lane has the mask of its node and takes those of its rows
+        bool wrong;
+        const uint64_t own_mask = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
+        if (wid == 0) s_wrong[lane] = wrong;
+        uint64_t mask[RT];
+#pragma unroll
+        for (int q = 0; q < RT; ++q) {
+            const int node = min(row0 + q * 16 + r, rows - 1) / G;
+            mask[q] = (uint64_t)(uint32_t)__shfl((uint32_t)(own_mask >> 32), node) << 32 | (uint32_t)__shfl((uint32_t)own_mask, node);
+        }
         for (t = j.t0 + wid; t < j.t1; t += 4) {
             const int node0 = (t - j.n_pre) * KT;
             if (t < j.n_pre || node0 >= j.count) continue;
@@ -541,7 +558,8 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
         l += __shfl_xor(l, 32);
         if (g == 0) { s_m[wid][t * 16 + r] = st.m[t]; s_l[wid][t * 16 + r] = l; }
     }
-    __syncthreads();
+    if (__syncthreads_or(bad)) j.ok = 2;
+    if (j.ok == 1 && a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
     const bool whole = j.whole;
     float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (RT * 16) * (D + 2);
     const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
@@ -622,20 +640,23 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     extern __shared__ __attribute__((aligned(1024))) char lds[];            // RING x (keys, values)
     __shared__ TreeJob s_job;
     __shared__ uint64_t s_mask[64];
-    __shared__ int s_wrong[64];
+    __shared__ int s_wrong[64], s_bad;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
     const bool late = wid >= TRW / 2;
     TreeJob j;
     for (bool first = true;; first = false) {
     TREE_ARGS(ka);
-    if (!tree_next<KT, ONE>(c, a, p, &s_job, j, first)) break;
+    if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j)) break; }
+    else if (!tree_next<KT>(c, a, p, &s_job, j, first)) break;
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, part_row0 = ((wid & 3) * 2 + (wid >> 2)) * 16 * RT, row0 = j.rb * TRW * 16 * RT + part_row0;
     if (wid == 0 && j.ok == 1) {
         bool wrong;
         const uint64_t m = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
         s_mask[lane] = m; s_wrong[lane] = wrong;
     }
+    if (tid == 0) { s_bad = 0; if (ONE) s_job = j; }
     __syncthreads();
+    if (j.ok == 1 && tree_bad(c, a, p, j, KT)) s_bad = 1;                          // (read behind later barriers)
     const int seq = __builtin_amdgcn_readfirstlane(j.seq), kh = __builtin_amdgcn_readfirstlane(j.kh), len = __builtin_amdgcn_readfirstlane(j.len);
     const int32_t* table = c.d_table + (int64_t)seq * c.max_pages;
     const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)kh * c.page_size * D;
@@ -643,7 +664,6 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     st.init();
     const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
     if (j.ok == 1) {
-        if (a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
         Frag qf[RT][KS];
         const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
 #pragma unroll
@@ -667,7 +687,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
         int pages = 0;
         auto page_of = [&](int t) {
             if ((t & 63) == 0) {
-                pages = table[min((t0 + min(t + lane, n_tiles - 1)) * KT + wid * RPW, len - 1) >> p.shift];
+                pages = page_ok(c, table[min((t0 + min(t + lane, n_tiles - 1)) * KT + wid * RPW, len - 1) >> p.shift]);
                 __builtin_amdgcn_s_waitcnt(0x0f70);                                // vmcnt(0): here, not by the compiler in every tile
             }
             return __builtin_amdgcn_readlane(pages, t & 63);
@@ -875,7 +895,10 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
             if (any_odd) add_odd_values<T, D, RT, NS>(c, a, p, j, table, head_off, page_e, 0, s, mask, st, g, r);
         }
     }
+    __syncthreads();
     j = s_job;
+    if (j.ok == 1 && s_bad) j.ok = 2;
+    if (j.ok == 1 && a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
     const bool whole = j.whole;
     float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (TRW * 16 * RT) * (D + 2);
 #pragma unroll
