@@ -87,7 +87,11 @@ class Case:
 @pytest.mark.parametrize("lens,N,heads,kv_heads,D,PS", [
     ([0], 1, 1, 1, 64, 16), ([1], 1, 2, 1, 64, 16), ([0, 5], 3, 2, 2, 64, 16), ([15, 16, 17], 7, 6, 6, 64, 16), ([31, 64, 65, 100], 16, 4, 2, 64, 32),
     ([300, 1, 77], 24, 20, 20, 64, 16), ([447] * 3, 1, 20, 20, 64, 16), ([200, 513], 64, 8, 2, 128, 64), ([129], 33, 16, 1, 128, 16),
-    ([1000, 63], 17, 6, 2, 128, 128), ([700], 5, 12, 4, 64, 256), ([2500, 3], 2, 3, 3, 128, 16)])
+    ([1000, 63], 17, 6, 2, 128, 128), ([700], 5, 12, 4, 64, 256), ([2500, 3], 2, 3, 3, 128, 16),
+    # every kernel and both of its ways of cutting the work: rows of a key / value head x head size x short and long contexts
+    ([90, 200], 24, 3, 3, 64, 16), ([1500, 20, 900], 24, 3, 3, 64, 16), ([100], 60, 2, 1, 64, 32), ([1400, 700], 60, 2, 1, 64, 32),
+    ([33, 129], 50, 8, 2, 64, 16), ([1300, 40], 50, 8, 2, 64, 16), ([60, 5], 20, 4, 4, 128, 16), ([1100, 64], 20, 4, 4, 128, 16),
+    ([65, 200], 40, 8, 2, 128, 32), ([4000], 40, 8, 2, 128, 32), ([130], 64, 16, 2, 128, 16), ([900, 2000], 64, 16, 2, 128, 64), ([50], 64, 16, 1, 64, 16)])
 @pytest.mark.parametrize("append", [True, False])
 def test_against_64_bits(dtype, lens, N, heads, kv_heads, D, PS, append):
     c = Case(lens, N, heads, kv_heads, D, PS, dtype, append=append, seed=N + len(lens))

@@ -156,6 +156,13 @@ __device__ __forceinline__ bool tree_next(const wx_cache& c, const wx_tree_attn&
     if (j.ok < 0) return false;
     return true;
 }
+// A job's numbers are alike on every lane: in scalar registers (read back from LDS they would take a vector register each, and every loop
+// over them a mask).
+__device__ __forceinline__ void tree_uniform(TreeJob& t) {
+#define UNI(x) t.x = __builtin_amdgcn_readfirstlane(t.x)
+    UNI(ok); UNI(i); UNI(kh); UNI(rb); UNI(piece); UNI(whole); UNI(seq); UNI(len); UNI(count); UNI(n_pre); UNI(t0); UNI(t1); UNI(last);
+#undef UNI
+}
 // The one job of a workgroup that does one whole sequence: no search, and nothing waits for another wave.
 template <int KT>
 __device__ __forceinline__ bool tree_whole(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob& t) {
@@ -352,26 +359,37 @@ __device__ __forceinline__ void add_odd_values(const wx_cache& c, const wx_tree_
             x = __shfl(x, ((k % 16) / 4) * 16 + r);
             const bool seen = (mask[t] >> (node0 + k)) & 1;
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d)
+            for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj) {
                     const float v = (float)row[16 * d + 4 * g + jj];
                     if (seen && !(fabsf(v) < INFINITY)) st.o[d][t][jj] = fmaf(x, v, st.o[d][t][jj]);
                 }
+                __builtin_amdgcn_sched_barrier(0);                                 // rare: no registers for its sake
+            }
         }
     }
 }
 
-// drafted rows -> the cache (one workgroup a sequence and head does it)
+// drafted rows -> the cache (one workgroup a sequence and head does it): 16 bytes a thread, the first of them loaded ahead
 template <typename T, int D>
-__device__ __forceinline__ void append_nodes(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off, int64_t page_e) {
+__device__ __forceinline__ i32x4 append_load(const wx_cache& c, const wx_tree_attn& a, const TreeJob& j, int u) {
     constexpr int E = 16 / sizeof(T), PER = D / E;
-    for (int u = threadIdx.x; u < j.count * PER * 2; u += blockDim.x) {
-        const int x = u % PER, node = (u / PER) % j.count, t = j.len + node;
-        const bool keys = u < j.count * PER;
-        T* to = reinterpret_cast<T*>(keys ? c.d_k : c.d_v) + head_off + table[t >> p.shift] * page_e + (int64_t)(t & (c.page_size - 1)) * D + x * E;
-        *reinterpret_cast<i32x4*>(to) = *reinterpret_cast<const i32x4*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, keys, node) + x * E);
-    }
+    const int x = u % PER, node = (u / PER) % j.count;
+    const T* row = u < j.count * PER ? reinterpret_cast<const T*>(a.d_kn) + j.i * a.kn_seq + node * a.kn_node + j.kh * a.kn_head
+                                     : reinterpret_cast<const T*>(a.d_vn) + j.i * a.vn_seq + node * a.vn_node + j.kh * a.vn_head;
+    return *reinterpret_cast<const i32x4*>(row + x * E);
+}
+template <typename T, int D>
+__device__ __forceinline__ T* append_place(const wx_cache& c, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off, int64_t page_e, int u) {
+    constexpr int E = 16 / sizeof(T), PER = D / E;
+    const int x = u % PER, node = (u / PER) % j.count, t = j.len + node;
+    return reinterpret_cast<T*>(u < j.count * PER ? c.d_k : c.d_v) + head_off + page_ok(c, table[t >> p.shift]) * page_e + (int64_t)(t & (c.page_size - 1)) * D + x * E;
+}
+template <typename T, int D>
+__device__ __forceinline__ void append_nodes(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off, int64_t page_e, int u0) {
+    constexpr int PER = D * (int)sizeof(T) / 16;
+    for (int u = u0; u < j.count * PER * 2; u += blockDim.x) *reinterpret_cast<i32x4*>(append_place<T, D>(c, p, j, table, head_off, page_e, u)) = append_load<T, D>(c, a, j, u);
 }
 
 template <typename T> __device__ __forceinline__ void store4(T* to, f32x4 v);
@@ -397,14 +415,18 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
     __shared__ TreeJob s_job;
     __shared__ int s_wrong[64];
     __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, r = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
     TreeJob j;
     for (bool first = true;; first = false) {
     TREE_ARGS(ka);
     if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j)) break; }
     else if (!tree_next<KT>(c, a, p, &s_job, j, first)) break;
+    tree_uniform(j);
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * RT * 16;
     int bad = 0;
+    const bool writes = j.ok == 1 && a.d_kn && j.rb == 0 && j.last;
+    i32x4 row0_part = {0, 0, 0, 0};
+    T* place = nullptr;
     const int32_t* table = c.d_table + (int64_t)j.seq * c.max_pages;
     const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)j.kh * c.page_size * D;
     RowState<D, RT> st;
@@ -430,35 +452,39 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
         char* vb = lds + wid * VBYTES;
         Frag kf[NS][KS], vr[NV];
         // a tile's pages: one for each 16 tokens, on lanes 0 .. NS-1
-        auto load_ids = [&](int t) { return page_ok(c, table[min(t * KT + 16 * min(lane, NS - 1), j.len - 1) >> p.shift]); };
+        auto load_ids = [&](int t) { return table[min(t * KT + 16 * min(lane, NS - 1), j.len - 1) >> p.shift]; };
+        // (a scalar base for the page and a 32-bit lane offset inside it: a page of one head is at most 128 KiB)
         auto load_pre = [&](int t, int ids) {
             const int last = j.len - 1 - t * KT;                                  // >= 0
+            ids = page_ok(c, ids);                                                // (here: looked at where it was loaded, it would be waited for there)
 #pragma unroll
             for (int k = 0; k < NS; ++k) {
-                const int64_t page = (int64_t)__builtin_amdgcn_readlane(ids, k) * page_e;
-                const int at = min(16 * k + r, last), base = t * KT + at;
-                const T* kr = Kp + page + (int64_t)(base & (c.page_size - 1)) * D;
+                const char* page = reinterpret_cast<const char*>(Kp + (int64_t)__builtin_amdgcn_readlane(ids, k) * page_e);
+                const uint32_t off = (((t * KT + min(16 * k + r, last)) & (c.page_size - 1)) * D + g * E) * (uint32_t)sizeof(T);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kf[k][ks] = *reinterpret_cast<const Frag*>(kr + (ks * 4 + g) * E);
+                for (int ks = 0; ks < KS; ++ks) kf[k][ks] = *reinterpret_cast<const Frag*>(page + (off + ks * 64));
             }
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 constexpr int RPL = 64 / CPR;                                     // rows a load covers
-                const int row = v * RPL + lane / CPR, at = min(row, last), base = t * KT + at;
-                const int64_t page = (int64_t)__builtin_amdgcn_readlane(ids, v * RPL / 16) * page_e;
-                vr[v] = *reinterpret_cast<const Frag*>(Vp + page + (int64_t)(base & (c.page_size - 1)) * D + (lane % CPR) * E);
+                const char* page = reinterpret_cast<const char*>(Vp + (int64_t)__builtin_amdgcn_readlane(ids, v * RPL / 16) * page_e);
+                const uint32_t off = (((t * KT + min(v * RPL + lane / CPR, last)) & (c.page_size - 1)) * D + (lane % CPR) * E) * (uint32_t)sizeof(T);
+                vr[v] = *reinterpret_cast<const Frag*>(page + off);
             }
         };
-        auto load_tree = [&](int node0) {
+        auto load_tree = [&](int node0) {                                         // (one address at a time in registers)
 #pragma unroll
             for (int k = 0; k < NS; ++k) {
                 const T* kr = node_row<T, D>(c, a, p, j, table, head_off, page_e, true, min(node0 + 16 * k + r, j.count - 1));
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) kf[k][ks] = *reinterpret_cast<const Frag*>(kr + (ks * 4 + g) * E);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+            for (int v = 0; v < NV; ++v) {
                 vr[v] = *reinterpret_cast<const Frag*>(node_row<T, D>(c, a, p, j, table, head_off, page_e, false, min(node0 + (v * 64 + lane) / CPR, j.count - 1)) + (lane % CPR) * E);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         // rows of the tile from `live` on are no tokens: their values count as 0 (their scores are masked)
         auto stage = [&](int live) {
@@ -482,8 +508,46 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
                     s[k][t] = x;
                 }
         };
+        // The drafted rows come first, the last wave's first tile: their places (where the call brings them) depend on no other load, so they are
+        // on their way while the length and the pages are looked up.  Every lane has the mask of its node and takes those of its rows.
+        bool wrong = a.d_parents && a.n_nodes == 1 && a.d_parents[j.i] != -1;
+        const uint64_t own_mask = a.n_nodes == 1 ? 1 : tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
+        if (wid == 0) s_wrong[lane] = wrong;
+        uint64_t mask[RT];
+#pragma unroll
+        for (int q = 0; q < RT; ++q) {
+            const int node = min(row0 + q * 16 + r, rows - 1) / G;
+            mask[q] = (uint64_t)(uint32_t)__shfl((uint32_t)(own_mask >> 32), node) << 32 | (uint32_t)__shfl((uint32_t)own_mask, node);
+        }
+        const int nt0 = ONE ? 0 : max(0, j.t0 - j.n_pre), nt1 = ONE ? p.tree_tiles : j.t1 - j.n_pre;
+        for (int nt = nt0 + 3 - wid; nt < nt1; nt += 4) {
+            const int node0 = nt * KT;
+            if (node0 >= j.count) break;
+            f32x4 s[NS][RT];
+            load_tree(node0);
+            bool odd = false;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) odd |= Elem<T>::odd(vr[v]);
+            const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+            if (any_odd)
+#pragma unroll
+                for (int v = 0; v < NV; ++v) vr[v] = finite_only(vr[v]);
+            stage(j.count - node0);
+            scores(s);
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) if (!((mask[q] >> (node0 + 16 * k + 4 * g + x)) & 1)) s[k][q][x] = -INFINITY;
+            st.template softmax<NS>(s, cc);
+            st.template add<NS, VROW>(s, vb, g, r, T());
+            if (any_odd) add_odd_values<T, D, RT, NS>(c, a, p, j, table, head_off, page_e, node0, s, mask, st, g, r);
+            __builtin_amdgcn_wave_barrier();
+        }
         const int end = min(j.t1, j.n_pre);
         int t = j.t0 + wid;
+        if (writes && tid < j.count * CPR * 2) { row0_part = append_load<T, D>(c, a, j, tid); place = append_place<T, D>(c, p, j, table, head_off, page_e, tid); }
         if (t >= end) bad = tree_bad(c, a, p, j, KT);
         else {
             int ids = load_ids(t);
@@ -514,41 +578,6 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
                 __builtin_amdgcn_wave_barrier();
             }
         }
-        // the drafted rows' tiles go on in the same rotation of waves; every lane has the mask of its node and takes those of its rows
-        bool wrong;
-        const uint64_t own_mask = tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
-        if (wid == 0) s_wrong[lane] = wrong;
-        uint64_t mask[RT];
-#pragma unroll
-        for (int q = 0; q < RT; ++q) {
-            const int node = min(row0 + q * 16 + r, rows - 1) / G;
-            mask[q] = (uint64_t)(uint32_t)__shfl((uint32_t)(own_mask >> 32), node) << 32 | (uint32_t)__shfl((uint32_t)own_mask, node);
-        }
-        for (t = j.t0 + wid; t < j.t1; t += 4) {
-            const int node0 = (t - j.n_pre) * KT;
-            if (t < j.n_pre || node0 >= j.count) continue;
-            f32x4 s[NS][RT];
-            load_tree(node0);
-            bool odd = false;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) odd |= Elem<T>::odd(vr[v]);
-            const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-            if (any_odd)
-#pragma unroll
-                for (int v = 0; v < NV; ++v) vr[v] = finite_only(vr[v]);
-            stage(j.count - node0);
-            scores(s);
-#pragma unroll
-            for (int k = 0; k < NS; ++k)
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-#pragma unroll
-                    for (int q = 0; q < RT; ++q) if (!((mask[q] >> (node0 + 16 * k + 4 * g + x)) & 1)) s[k][q][x] = -INFINITY;
-            st.template softmax<NS>(s, cc);
-            st.template add<NS, VROW>(s, vb, g, r, T());
-            if (any_odd) add_odd_values<T, D, RT, NS>(c, a, p, j, table, head_off, page_e, node0, s, mask, st, g, r);
-            __builtin_amdgcn_wave_barrier();
-        }
     }
     // ---- the four waves' states: factors first, then 64 columns of the outputs at a time ---------------------------------------------
 #pragma unroll
@@ -558,8 +587,11 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
         l += __shfl_xor(l, 32);
         if (g == 0) { s_m[wid][t * 16 + r] = st.m[t]; s_l[wid][t * 16 + r] = l; }
     }
-    if (__syncthreads_or(bad)) j.ok = 2;
-    if (j.ok == 1 && a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
+    if (__builtin_amdgcn_readfirstlane(__syncthreads_or(bad))) j.ok = 2;
+    if (writes && j.ok == 1) {
+        if (tid < j.count * CPR * 2) *reinterpret_cast<i32x4*>(place) = row0_part;
+        append_nodes<T, D>(c, a, p, j, table, head_off, page_e, tid + 256);
+    }
     const bool whole = j.whole;
     float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (RT * 16) * (D + 2);
     const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
@@ -898,7 +930,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     __syncthreads();
     j = s_job;
     if (j.ok == 1 && s_bad) j.ok = 2;
-    if (j.ok == 1 && a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e);
+    if (j.ok == 1 && a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e, tid);
     const bool whole = j.whole;
     float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (TRW * 16 * RT) * (D + 2);
 #pragma unroll
@@ -1020,8 +1052,13 @@ struct TreeForm { bool rows_form; int rt, rows, kt; };
 static TreeForm tree_form(const wx_cache& c, const wx_tree_attn& a) {
     const int rows = a.n_nodes * (a.n_head / c.n_kv_head), es = c.precision == WX_PREC_F32 ? 4 : 2;
     TreeForm f;
-    f.rows_form = c.precision == WX_PREC_BF16 && rows > 64;
-    f.rt = f.rows_form ? rows > 128 ? 2 : 1 : rows > 16 ? 2 : 1;
+    // Both forms measured at contexts of 4000-16000 tokens and below 500.  Heads of 128: up to 16 rows the waves share the keys (14.7 us
+    // against 20.4 at 32 x 4 rows and short contexts; 164 against 150 at long ones), above that they share the rows (16 x 32 rows: 153 us
+    // against 171; 16 x 64 rows: 169 against 225).  Heads of 64, whose tiles are half as large for the same barriers: 16 x 64 rows 249 us with
+    // the keys shared, 487 with the rows.
+    f.rows_form = c.precision == WX_PREC_BF16 && rows > (c.head_dim == 128 ? 16 : 128);
+    // 32 rows a wave (two row tiles for every fragment read) where they are there and the registers allow it
+    f.rt = f.rows_form ? rows > 128 ? 2 : 1 : rows > 16 && c.head_dim == 64 ? 2 : 1;
     f.rows = f.rows_form ? 128 * f.rt : 16 * f.rt;
     f.kt = f.rows_form ? 64 : 8192 / (c.head_dim * es);
     return f;
@@ -1236,12 +1273,12 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
                               if (le != hipSuccess) return set_error(WX_ERR_HIP, hipGetErrorString(le)); } while (0)
     if (f.rows_form) {
         if (wide) { if (f.rt == 2) TREE_ROWS(128, 2); else TREE_ROWS(128, 1); }
-        else { if (f.rt == 2) TREE_ROWS(64, 2); else TREE_ROWS(64, 1); }
+        else TREE_ROWS(64, 2);
     } else if (f32) {
-        if (wide) { if (f.rt == 2) TREE_KEYS(float, 128, 2); else TREE_KEYS(float, 128, 1); }
+        if (wide) TREE_KEYS(float, 128, 1);
         else { if (f.rt == 2) TREE_KEYS(float, 64, 2); else TREE_KEYS(float, 64, 1); }
     } else {
-        if (wide) { if (f.rt == 2) TREE_KEYS(bf16, 128, 2); else TREE_KEYS(bf16, 128, 1); }
+        if (wide) TREE_KEYS(bf16, 128, 1);
         else { if (f.rt == 2) TREE_KEYS(bf16, 64, 2); else TREE_KEYS(bf16, 64, 1); }
     }
     if (!p.single) {

@@ -98,9 +98,6 @@ class PagedKVCache:
             raise ValueError(f"{what} requires a gradient: the cache's operators have none (detach it)")
         return t if t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
 
-    def _status(self, n: int) -> torch.Tensor:
-        return torch.empty(n, dtype=torch.int32, device=self.device)
-
     # -- pages --------------------------------------------------------------------------------------------
     def truncate(self, seqs, lens=None) -> torch.Tensor:
         """Slot ``seqs[i]`` keeps its first ``lens[i]`` tokens (None: none, the slot is freed) and gives up the pages behind them.
@@ -109,7 +106,7 @@ class PagedKVCache:
         n = seqs.shape[0]
         if lens is not None:
             lens = self._ids(lens, "lens", n)
-        status = self._status(n)
+        status = torch.empty_like(seqs)
         _check(self.lib.wx_cache_truncate(self._ref, seqs.data_ptr(), None if lens is None else lens.data_ptr(), n, status.data_ptr(),
                                           _raw_stream(self._index)), "wx_cache_truncate")
         return status
@@ -124,7 +121,7 @@ class PagedKVCache:
         dst = self._ids(dst, "dst")
         n = dst.shape[0]
         src = self._ids(src, "src", n)
-        status = self._status(n)
+        status = torch.empty_like(dst)
         _check(self.lib.wx_cache_fork(self._ref, dst.data_ptr(), src.data_ptr(), n, status.data_ptr(), _raw_stream(self._index)), "wx_cache_fork")
         return status
 
@@ -134,7 +131,7 @@ class PagedKVCache:
         seqs = self._ids(seqs, "seqs")
         n = seqs.shape[0]
         each = None if isinstance(extra, int) else self._ids(extra, "extra", n)
-        status = self._status(n)
+        status = torch.empty_like(seqs)
         _check(self.lib.wx_cache_reserve(self._ref, seqs.data_ptr(), None if each is None else each.data_ptr(), extra if each is None else 0, n,
                                          status.data_ptr(), _raw_stream(self._index)), "wx_cache_reserve")
         return status
@@ -164,7 +161,7 @@ class PagedKVCache:
         counts = self._ids(counts, "counts", n)
         nodes = path.shape[-1] if torch.is_tensor(path) else -1
         path = self._ids(path, "path", n, nodes)
-        status = self._status(n)
+        status = torch.empty_like(seqs)
         _check(self.lib.wx_cache_commit(self._ref, seqs.data_ptr(), path.data_ptr(), counts.data_ptr(), n, nodes, status.data_ptr(),
                                         _raw_stream(self._index)), "wx_cache_commit")
         return status
@@ -200,7 +197,7 @@ class PagedKVCache:
         if counts is not None:
             counts = self._ids(counts, "counts", n)
         if out is None:
-            out = torch.empty((n, nodes, heads, self.head_dim), dtype=self.dtype, device=self.device)
+            out = torch.empty_like(q)
         elif self._rows(out, "out", (n, nodes, heads, self.head_dim)) is not out:
             raise ValueError("out's last dimension must be contiguous")
         a = _lib.WxTreeAttn(
