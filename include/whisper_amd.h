@@ -292,9 +292,9 @@ int wx_cache_compact(const wx_cache* c, int32_t* d_n_live, void* stream);
  * committed tokens, itself and its ancestors.  d_parents [n][n_nodes]: the parent of node i, < i, or -1 where it follows the
  * committed tokens directly (NULL: a chain).  d_counts[i] (NULL: n_nodes) nodes are there; the rows of the others, and of a sequence
  * id -1 (padding of a batch), come out as 0.  With d_kn / d_vn the nodes' keys and values are appended behind the committed tokens by the same
- * call (as wx_cache_append does; the ids must be distinct then), without (both NULL) they lie there.  A sequence id out of range, rows that are not reserved, a
- * second entry of the same id in an appending call, or a parent out of range (and its descendants) give rows of NaN and append
- * nothing.  n_nodes == 1 is the ordinary decode step.  n_head: query heads, a multiple of n_kv_head up to 16 x as many; head h reads key/value head
+ * call (as wx_cache_append does; the ids must be distinct then), without (both NULL) they lie there.  A sequence id out of range, rows that are not reserved or
+ * whose pages another slot holds too, and a second entry of the same id in an appending call give rows of NaN and append nothing; so do
+ * the rows of a sequence with a page number outside the pool, and of a node with a parent out of range and its descendants.  n_nodes == 1 is the ordinary decode step.  n_head: query heads, a multiple of n_kv_head up to 16 x as many; head h reads key/value head
  * h / (n_head / n_kv_head).  Strides in elements: heads' rows are contiguous and 16-byte aligned.  Softmax and sums in fp32; bf16
  * caches round the probabilities to bf16 for the product with the values.  What masked rows hold (NaN, infinities) has no effect.
  * split_tokens: the committed tokens are cut into pieces that workgroups take side by side; 0 = by the size of the batch; > 0 = pieces
@@ -329,6 +329,25 @@ typedef struct {
 } wx_tree_check;
 int64_t wx_tree_verify_work_bytes(const wx_tree_check* a);
 int wx_tree_verify(const wx_tree_check* a, void* stream);
+
+/* one pass of this engine's decoder over drafted tokens, on the caller's cache: entry i is the sequence in cache slot d_seqs[i], which
+ * listens to window i / group of the last wx_encode.  Its nodes (d_tokens, d_parents, d_counts as wx_tree_attn; n_nodes <= 64; a prompt is
+ * a chain) stand at the positions behind the committed tokens, by depth; their keys and values are appended to the cache in every layer, and
+ * row (i, j) of d_logits [n][n_nodes][wx_logit_stride()] receives what the model answers to node j (want_logits 0: nothing, the pass
+ * only fills the cache, as for a prompt).  Slots have to be reserved n_nodes tokens ahead.  The lengths stay: wx_tree_verify and
+ * wx_cache_commit follow (WhisperEngine.decode_draft is the whole loop).  The cache has the engine's precision and device, n_text_layer
+ * layers, n_text_head heads of 64, and at most 512 tokens a slot, so that a sequence's numbers do not depend on what else is in the pass.
+ * Positions past n_text_ctx - 1 are not embedded: keep the depth within them.  Serves upstream's greedy DecodingTask.run (inside
+ * ref:speech_recognition.py:55), several tokens a pass. */
+typedef struct {
+    int32_t n, n_nodes, group, want_logits;
+    const int32_t *d_seqs, *d_tokens, *d_parents, *d_counts;   /* [n], [n][n_nodes], [n][n_nodes] or NULL (chains), [n] or NULL */
+    float* d_logits;
+    void* d_work; int64_t work_bytes;                          /* wx_draft_work_bytes(), 256-byte aligned; contents are never kept */
+} wx_draft_pass;
+int32_t wx_logit_stride(wx_engine* e);                         /* floats a row of d_logits: n_vocab rounded up to 16 */
+int64_t wx_draft_work_bytes(wx_engine* e, int32_t n, int32_t n_nodes);
+int wx_draft_logits(wx_engine* e, const wx_cache* c, const wx_draft_pass* p, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,188 @@
+"""Drafted decoding of the engine (wx_draft_logits, WhisperEngine.decode_draft): the drafted nodes' logits against the decoder's own,
+position by position, and greedy's ids whatever the drafts."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import whisper_oracle as wo
+from whisper_amd import checkpoint as ck
+from whisper_amd.draft import EngineDraft, NgramDraft
+
+pytestmark = pytest.mark.gpu
+
+
+def make(precision="fp32", max_batch=4, name="micro", windows=3, eot_boost=1.0, **kw):
+    from whisper_amd.engine import WhisperEngine
+    dims = ck.dims_for(name)
+    eng = WhisperEngine(dims, ck.synthetic_state_dict(dims, seed=0, eot_boost=eot_boost), precision=precision, max_batch=max_batch, **kw)
+    audio = torch.from_numpy(np.concatenate([wo.varied_audio(i, 16000 * 30) for i in range(windows)])).cuda()
+    mel = eng.log_mel(audio)
+    encode = lambda e: e.encode(mel, 3000, mel.stride(0), audio.numel() // 160, min(windows, max_batch))  # noqa: E731
+    encode(eng)
+    return eng, mel, encode
+
+
+def prompts(eng, extra=((), (5, 6, 7), (11, 12))):
+    base = eng.initial_tokens(0)
+    return [[eng.tok.sot_prev, *e, *base] if e else list(base) for e in extra]
+
+
+class Given:
+    """drafts made from each row's whole greedy text: right, wrong from some id on, or mixed with wrong branches"""
+
+    def __init__(self, full, kind, seed=0):
+        self.full, self.kind, self.rng = full, kind, np.random.RandomState(seed)
+
+    def __call__(self, rows, k):
+        out = []
+        for ids, full in zip(rows, self.full):
+            true = full[len(ids):len(ids) + k]
+            wrong = self.rng.randint(0, 300, k).tolist()
+            out.append({"none": [], "right": [true], "wrong": [wrong], "empty": [[]],
+                        "mixed": [wrong, true[:2] + wrong, true, true]}[self.kind])
+        return out
+
+
+@pytest.mark.parametrize("kind", ["none", "right", "wrong", "mixed", "empty"])
+@pytest.mark.parametrize("n_nodes", [1, 7, 64])
+def test_ids_are_greedys_whatever_the_drafts(kind, n_nodes):
+    eng, _, _ = make()
+    try:
+        ps = prompts(eng)
+        want = eng.decode_rows(ps, max_new_tokens=40)
+        full = [p + t + [eng.tok.eot] for p, t in zip(ps, want["tokens"])]
+        got = eng.decode_draft(ps, Given(full, kind), n_nodes=n_nodes, n_draft=6, max_new_tokens=40)
+        assert got["tokens"] == want["tokens"]
+        np.testing.assert_allclose(got["sum_logprobs"], want["sum_logprobs"], rtol=1e-4, atol=1e-3)      # the bars of the fp32 engine's own tests
+        np.testing.assert_allclose(got["no_speech_probs"], want["no_speech_probs"], rtol=1e-3, atol=1e-6)
+        longest = max(len(t) for t in want["tokens"])
+        if kind == "right" and n_nodes > 1:
+            assert got["passes"] <= 2 + -(-longest // min(n_nodes, 7)) and got["accepted"] > 0
+        if kind in ("none", "empty") or n_nodes == 1:
+            assert got["accepted"] == 0 and longest <= got["passes"] <= longest + 1
+    finally:
+        eng.close()
+
+
+def test_a_whole_context_and_ngrams():
+    """no end in sight: the rows run to the last position of the context, one of them from a long prompt"""
+    eng, _, _ = make(eot_boost=-50.0, windows=2)
+    try:
+        base = eng.initial_tokens(0)
+        ps = [list(base), [eng.tok.sot_prev] + [int(x) for x in np.random.RandomState(0).randint(0, 300, 200)] + list(base)]
+        for limit in (0, 446):
+            want = eng.decode_rows(ps, max_new_tokens=limit)
+            got = eng.decode_draft(ps, NgramDraft(3, 3), n_nodes=24, n_draft=12, max_new_tokens=limit)
+            assert got["tokens"] == want["tokens"]
+            np.testing.assert_allclose(got["sum_logprobs"], want["sum_logprobs"], rtol=1e-4, atol=1e-2)
+            assert got["passes"] <= max(len(t) for t in want["tokens"]) + 1
+    finally:
+        eng.close()
+
+
+def test_another_engines_drafts():
+    eng, _, encode = make(max_batch=4)
+    helper = eng.replica()
+    try:
+        encode(helper)
+        ps = prompts(eng)
+        want = eng.decode_rows(ps, max_new_tokens=30)
+        got = eng.decode_draft(ps, EngineDraft(helper), n_nodes=9, n_draft=8, max_new_tokens=30)
+        assert got["tokens"] == want["tokens"] and got["accepted"] > 0
+        longest = max(len(t) for t in want["tokens"])
+        assert got["passes"] <= 2 + -(-longest // 9) + 1                       # the same model: every draft agrees
+    finally:
+        helper.close()
+        eng.close()
+
+
+@pytest.mark.parametrize("precision,max_batch", [("fp32", 4), ("bf16", 4), ("bf16", 32)])
+def test_node_logits_against_the_decoder(precision, max_batch, monkeypatch):
+    """the logits of every node of a tree = the decoder's for the prompt and the path to the node; two entries listen to each window.  Drafted
+    passes attend cached cross K/V; an engine whose own decode attends the encoder output instead (bf16, 32 rows and up: other rounding
+    points) is held to the decoder of one that is made with cached K/V."""
+    eng, _, _ = make(precision, max_batch, windows=2)
+    ref = eng
+    if eng.cross_form != "kv":
+        monkeypatch.setenv("WX_NO_XATTN", "1")
+        ref, _, _ = make(precision, max_batch, windows=2)
+        assert ref.cross_form == "kv"
+    try:
+        rng = np.random.RandomState(1)
+        N, prompt = 7, rng.randint(0, 300, (4, 5)).astype(np.int32)
+        par = np.array([[-1, 0, 0, 1, 3, 2, -1]] * 4, np.int32)
+        tok = rng.randint(0, 300, (4, N)).astype(np.int32)
+        cache = eng.draft_cache(4)
+        i32 = lambda a: torch.tensor(np.ascontiguousarray(a), dtype=torch.int32, device="cuda")  # noqa: E731
+        slots = i32([2, 0, 3, 1])
+        cache.reserve(slots, 5)
+        assert eng.draft_logits(cache, slots, i32(prompt), group=2, want_logits=False) is None
+        cache.commit(slots, i32([[0, 1, 2, 3, 4]] * 4), i32([5] * 4))
+        cache.reserve(slots, N)
+        got = eng.draft_logits(cache, slots, i32(tok), i32(par), group=2).cpu().numpy()
+        again = eng.draft_logits(cache, slots, i32(tok), i32(par), group=2).cpu().numpy()
+        np.testing.assert_array_equal(got, again)
+        worst = 0.0
+        for e in range(4):
+            for j in range(N):
+                way, p = [], j
+                while p >= 0:
+                    way.append(int(tok[e, p]))
+                    p = int(par[e, p])
+                seq = [int(x) for x in prompt[e]] + way[::-1]
+                # entry e listens to window e // 2: decode both windows, read that one
+                want = ref.decoder_logits(torch.tensor([seq, seq]))[e // 2, -1].cpu().numpy()
+                worst = max(worst, float(np.abs(got[e, j] - want).max() / np.abs(want).max()))
+        # fp32: the bar of the engine's own logit tests; bf16: the activations of every layer are rounded to half a step of 2^-8 by both sides, at places
+        # that differ by the order of sums: a few such steps of the largest logit
+        assert worst < (1e-4 if precision == "fp32" else 6 * 2.0 ** -8), worst
+    finally:
+        if ref is not eng:
+            ref.close()
+        eng.close()
+
+
+def test_windows_path_with_ngram_drafts():
+    eng, mel, _ = make(max_batch=2, windows=3)
+    try:
+        init = eng.initial_tokens(0)
+        want = eng.transcribe_mel(mel, 9000, 0, 3, init, max_new_tokens=25)
+        got = eng.transcribe_mel(mel, 9000, 0, 3, init, max_new_tokens=25, draft="ngram")
+        assert got["tokens"] == want["tokens"]
+        np.testing.assert_allclose(got["sum_logprobs"], want["sum_logprobs"], rtol=1e-4, atol=1e-3)
+        with pytest.raises(ValueError):
+            eng.transcribe_mel(mel, 9000, 0, 3, init, draft="ngram", beam_size=2)
+        with pytest.raises(ValueError):
+            eng.transcribe_mel(mel, 9000, 0, 3, init, draft="other")
+    finally:
+        eng.close()
+
+
+def test_refusals():
+    from whisper_amd._lib import WxError
+    from whisper_amd.kvcache import PagedKVCache
+    eng, _, _ = make(windows=2)
+    try:
+        base = eng.initial_tokens(0)
+        for bad in ([[]], [[1, 2]], [base * 300], [base + [10 ** 7]]):
+            with pytest.raises(ValueError):
+                eng.decode_draft(bad)
+        for kw in (dict(without_timestamps=False), dict(n_nodes=0), dict(n_nodes=65), dict(n_draft=0)):
+            with pytest.raises(ValueError):
+                eng.decode_draft([base], **kw)
+        with pytest.raises(WxError, match="group"):
+            eng.decode_draft([base] * 3)                                       # three rows, two windows
+        i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+        cache = eng.draft_cache(2)
+        with pytest.raises(ValueError):
+            eng.draft_cache(2, 65)
+        with pytest.raises(ValueError):
+            eng.draft_logits(cache, i32([0]), i32([[1, 2]]), i32([[0]]))
+        other = PagedKVCache.allocate(1, eng.dims.n_text_head, 64, 8, 2, 4, dtype=torch.bfloat16)
+        with pytest.raises(WxError, match="precision"):
+            eng.draft_logits(other, i32([0]), i32([[1]]))
+        wide = PagedKVCache.allocate(eng.dims.n_text_layer, eng.dims.n_text_head, 64, 8, 2, 64, dtype=torch.float32)
+        with pytest.raises(WxError, match="512"):
+            eng.draft_logits(wide, i32([0]), i32([[1]]))
+    finally:
+        eng.close()

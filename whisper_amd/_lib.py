@@ -48,6 +48,11 @@ class WxTreeCheck(ctypes.Structure):
         ("d_work", c_vp), ("work_bytes", c_i64)]
 
 
+class WxDraftPass(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("n", "n_nodes", "group", "want_logits")] + [(n, c_vp) for n in (
+        "d_seqs", "d_tokens", "d_parents", "d_counts", "d_logits", "d_work")] + [("work_bytes", c_i64)]
+
+
 # name -> (restype, argtypes); exactly the declarations of include/whisper_amd.h
 PROTOTYPES = {
     "wx_last_error": (ctypes.c_char_p, []),
@@ -94,6 +99,9 @@ PROTOTYPES = {
     "wx_tree_attention": (c_i32, [c_vp, c_vp, c_vp]),
     "wx_tree_verify_work_bytes": (c_i64, [c_vp]),
     "wx_tree_verify": (c_i32, [c_vp, c_vp]),
+    "wx_logit_stride": (c_i32, [c_vp]),
+    "wx_draft_work_bytes": (c_i64, [c_vp, c_i32, c_i32]),
+    "wx_draft_logits": (c_i32, [c_vp, c_vp, c_vp, c_vp]),
 }
 
 _lib = None

@@ -306,6 +306,9 @@ struct OnDevice {
     }
     ~OnDevice() { if (prev >= 0 && prev != dev) (void)hipSetDevice(prev); }
 };
+// x[i * n_nodes + j][:] = tok_emb[tokens[i][j]][:] + pos_emb[length of slot seqs[i] + depth of node j][:] (ids and positions clamped to the tables)
+int launch_tree_embed(const void* tok_emb, const void* pos_emb, int dt, const wx_cache& c, const int32_t* seqs, const int32_t* tokens, const int32_t* parents,
+                      int n, int n_nodes, float* x, int d, hipStream_t st, int n_tok, int n_pos);
 // nullptr, or what is wrong with a cache's description (host-side check of every call)
 const char* cache_fault(const wx_cache* c);
 

@@ -1466,6 +1466,112 @@ int wx_decoder_logits(wx_engine* e, int32_t B, const int32_t* d_tokens, int32_t 
     return WX_OK;
 }
 
+// ---- drafted decoding on the caller's cache (include/whisper_amd.h: wx_draft_logits) -----------------------------------------------------
+// The decoder layers as decode_step_f32 has them (every GEMM applies its own epilogue), for n x n_nodes rows: self-attention is the tree
+// attention over the cache (which appends the rows' keys and values), cross-attention the encoder's kernels on the cached K/V, the rows
+// of a window being its queries.
+}  // extern "C"
+
+static size_t draft_round(size_t b) { return (b + 255) & ~(size_t)255; }
+struct DraftWork { float* x; char *xn, *qkv, *att, *hid, *q; size_t bytes; };
+static DraftWork draft_work(const wx_engine* e, int64_t rows, char* base) {
+    const size_t es = dtype_size(e->dt), d = e->d;
+    DraftWork w;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { char* p = base + at; at += draft_round(bytes); return p; };
+    w.x = (float*)take(rows * d * 4);
+    w.xn = take(rows * d * es); w.qkv = take(rows * 3 * d * es); w.att = take(rows * d * es); w.hid = take(rows * 4 * d * es); w.q = take(rows * d * es);
+    w.bytes = at;
+    return w;
+}
+
+extern "C" {
+
+int32_t wx_logit_stride(wx_engine* e) { return e ? e->vocab_pad : 0; }
+
+int64_t wx_draft_work_bytes(wx_engine* e, int32_t n, int32_t n_nodes) {
+    if (!e || n < 1 || n_nodes < 1 || n > 8192 || n_nodes > 64) return fail(WX_ERR_INVALID, "bad draft size");
+    return (int64_t)draft_work(e, (int64_t)n * n_nodes, nullptr).bytes;
+}
+
+int wx_draft_logits(wx_engine* e, const wx_cache* c, const wx_draft_pass* p, void* stream) {
+    if (!e || !e->finalized) return fail(WX_ERR_STATE, "engine not finalized");
+    if (const char* m = cache_fault(c)) return fail(WX_ERR_INVALID, m);
+    if (!p || !p->d_seqs || !p->d_tokens || !p->d_work || (p->want_logits && !p->d_logits)) return fail(WX_ERR_INVALID, "null argument");
+    const wx_config& k = e->cfg;
+    if (c->precision != k.precision || c->device != k.device || c->n_layer != k.n_text_layer || c->n_kv_head != e->Ht || c->head_dim != HEAD_DIM)
+        return fail(WX_ERR_INVALID, "the cache's precision, device, layers or heads are not this decoder's");
+    if ((int64_t)c->max_pages * c->page_size > 512) return fail(WX_ERR_INVALID, "the cache must hold at most 512 tokens a slot");
+    if (p->n_nodes < 1 || p->n_nodes > 64) return fail(WX_ERR_INVALID, "n_nodes must be 1 .. 64");
+    if (p->n < 1 || p->n > 8192 || p->group < 1 || p->n % p->group || p->n / p->group > e->encoded_B) return fail(WX_ERR_INVALID, "entries must be whole groups, one for each window of the last wx_encode at most");
+    const int64_t rows64 = (int64_t)p->n * p->n_nodes;
+    if (p->work_bytes < wx_draft_work_bytes(e, p->n, p->n_nodes) || ((uintptr_t)p->d_work & 255)) return fail(WX_ERR_INVALID, "work buffer too small or not 256-byte aligned");
+    if ((uintptr_t)p->d_logits & 15) return fail(WX_ERR_INVALID, "logits must be 16-byte aligned");
+    DeviceScope dev_scope(e);
+    hipStream_t st = (hipStream_t)stream;
+    const int d = e->d, dtp = e->dt, T = e->T, R = (int)rows64, windows = p->n / p->group, per_window = p->group * p->n_nodes;
+    const size_t es = dtype_size(dtp);
+    if (!e->crossK || (e->xattn && e->cross_kv_B < windows)) { if (int r = project_cross_kv(e, e->encoded_B, st)) return r; }
+    const DraftWork w = draft_work(e, R, (char*)p->d_work);
+    const size_t cross_layer = (size_t)k.max_batch * e->Ht * T * HEAD_DIM;
+    WX_TRY(launch_tree_embed(e->tok_emb, e->dec_pos, dtp, *c, p->d_seqs, p->d_tokens, p->d_parents, p->n, p->n_nodes, w.x, d, st, k.n_vocab, k.n_text_ctx));
+    for (int i = 0; i < k.n_text_layer; ++i) {
+        const LayerW& L = e->dec[i];
+        auto gemm = [&](const void* A, int64_t lda, const void* W, int N, int K, const float* bias, void* out, int out_dt, int64_t ldo) {
+            GemmArgs g = gemm_basic(e, A, lda, W, R, N, K);
+            g.ep.bias = bias; g.ep.out = out; g.ep.out_dtype = out_dt; g.ep.ldo = ldo;
+            return g;
+        };
+        auto residual = [&](GemmArgs g) { g.ep.residual = w.x; g.ep.ldr = d; return launch_gemm(g, st); };
+        WX_TRY(launch_layernorm(w.x, L.ln1_g, L.ln1_b, w.xn, dtp, R, d, st));
+        {
+            GemmArgs g = gemm(w.xn, d, L.self.wqkv, 3 * d, d, L.self.bqkv, w.qkv, dtp, 3 * d);
+            g.ep.colscale_period = d; g.ep.colscale[0] = e->qk_scale; g.ep.colscale[1] = e->qk_scale;
+            WX_TRY(launch_gemm(g, st));
+        }
+        {
+            wx_tree_attn a{};
+            a.layer = i; a.n = p->n; a.n_nodes = p->n_nodes; a.n_head = e->Ht;
+            a.d_seqs = p->d_seqs; a.d_parents = p->d_parents; a.d_counts = p->d_counts;
+            a.d_q = w.qkv; a.d_kn = w.qkv + (size_t)d * es; a.d_vn = w.qkv + (size_t)2 * d * es; a.d_out = w.att;
+            a.q_seq = a.kn_seq = a.vn_seq = (int64_t)p->n_nodes * 3 * d; a.q_node = a.kn_node = a.vn_node = 3 * d;
+            a.q_head = a.kn_head = a.vn_head = a.o_head = HEAD_DIM;
+            a.o_seq = (int64_t)p->n_nodes * d; a.o_node = d;
+            a.scale = 1.f;                                                    // q and k carry head_dim^-0.25 each
+            if (int r = wx_tree_attention(c, &a, stream)) return r;
+        }
+        WX_TRY(residual(gemm(w.att, d, L.self.wo, d, d, L.self.bo, w.x, DT_F32, d)));
+        WX_TRY(launch_layernorm(w.x, L.lnx_g, L.lnx_b, w.xn, dtp, R, d, st));
+        {
+            GemmArgs g = gemm(w.xn, d, L.xq, d, d, L.xbq, w.q, dtp, d);
+            g.ep.colscale_period = d; g.ep.colscale[0] = e->qk_scale;
+            WX_TRY(launch_gemm(g, st));
+        }
+        {
+            AttnArgs a;
+            a.dt = dtp; a.Q = w.q; a.q_sb = (int64_t)per_window * d; a.q_sq = d; a.q_sh = HEAD_DIM; a.n_q = per_window;
+            a.K = (char*)e->crossK + cross_layer * i * es; a.V = (char*)e->crossV + cross_layer * i * es; a.kv_sbh = (int64_t)T * HEAD_DIM; a.n_keys = T;
+            a.O = w.att; a.o_sb = (int64_t)per_window * d; a.o_sq = d; a.o_sh = HEAD_DIM; a.B = windows; a.H = e->Ht;
+            WX_TRY(dtp == DT_BF16 ? launch_attn_flash_bf16(a, st) : launch_attn_rows(a, st));
+        }
+        WX_TRY(residual(gemm(w.att, d, L.xo, d, d, L.xbo, w.x, DT_F32, d)));
+        WX_TRY(launch_layernorm(w.x, L.ln2_g, L.ln2_b, w.xn, dtp, R, d, st));
+        {
+            GemmArgs g = gemm(w.xn, d, L.w1, 4 * d, d, L.b1, w.hid, dtp, 4 * d);
+            g.ep.act = 1;
+            WX_TRY(launch_gemm(g, st));
+        }
+        WX_TRY(residual(gemm(w.hid, 4 * d, L.w2, d, 4 * d, L.b2, w.x, DT_F32, d)));
+    }
+    if (!p->want_logits) return WX_OK;
+    WX_TRY(launch_layernorm(w.x, e->declnf_g, e->declnf_b, w.xn, dtp, R, d, st));
+    GemmArgs g = gemm_basic(e, w.xn, d, e->tok_emb, R, e->vocab_pad, d);
+    g.Wpk = e->tok_emb_pk;
+    g.ep.out = p->d_logits; g.ep.out_dtype = DT_F32; g.ep.ldo = e->vocab_pad;
+    WX_TRY(launch_gemm(g, st));
+    return WX_OK;
+}
+
 int64_t wx_weight_bytes(wx_engine* e) { return e && e->owns_weights ? e->weight_bytes : 0; }
 int64_t wx_workspace_bytes(wx_engine* e) { return e ? e->work_bytes : 0; }
 int32_t wx_cross_attention_form(wx_engine* e) { return e && e->xattn ? 1 : 0; }

@@ -1087,6 +1087,32 @@ static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {
     return (int64_t)p.pieces * c.n_kv_head * p.row_blocks * p.rows * (c.head_dim + 2) * 4;
 }
 
+// ---- the decoder's input for drafted tokens: one workgroup a node ------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void tree_embed_kernel(const T* tok_emb, const T* pos_emb, wx_cache c, const int32_t* seqs, const int32_t* tokens, const int32_t* parents,
+                                                         int n_nodes, float* x, int d, int n_tok, int n_pos) {
+    const int i = blockIdx.x / n_nodes, j = blockIdx.x % n_nodes, s = seqs[i];
+    int depth = j;
+    if (parents) {
+        depth = 0;
+        for (int at = j, up = parents[(int64_t)i * n_nodes + j]; up >= 0 && up < at; ++depth) { at = up; up = parents[(int64_t)i * n_nodes + at]; }
+    }
+    int t = depth + (s >= 0 && s < c.max_seqs ? c.d_lens[s] : 0);
+    if (t > n_pos - 1) t = n_pos - 1;
+    if (t < 0) t = 0;
+    int token = tokens[blockIdx.x];
+    if ((unsigned)token >= (unsigned)n_tok) token = n_tok - 1;
+    const T *te = tok_emb + (int64_t)token * d, *pe = pos_emb + (int64_t)t * d;
+    for (int q = threadIdx.x; q < d; q += 256) x[(int64_t)blockIdx.x * d + q] = (float)te[q] + (float)pe[q];
+}
+int launch_tree_embed(const void* tok_emb, const void* pos_emb, int dt, const wx_cache& c, const int32_t* seqs, const int32_t* tokens, const int32_t* parents,
+                      int n, int n_nodes, float* x, int d, hipStream_t st, int n_tok, int n_pos) {
+    if (n < 1 || n_nodes < 1 || n_tok < 1 || n_pos < 1) return -1;
+    if (dt == DT_F32) hipLaunchKernelGGL(tree_embed_kernel<float>, dim3(n * n_nodes), dim3(256), 0, st, (const float*)tok_emb, (const float*)pos_emb, c, seqs, tokens, parents, n_nodes, x, d, n_tok, n_pos);
+    else hipLaunchKernelGGL(tree_embed_kernel<bf16>, dim3(n * n_nodes), dim3(256), 0, st, (const bf16*)tok_emb, (const bf16*)pos_emb, c, seqs, tokens, parents, n_nodes, x, d, n_tok, n_pos);
+    return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
 // ---- verification ---------------------------------------------------------------------------------------------------------------------
 struct Best { float m, s; int i; };       // largest logit, sum of exp(logit - m), its lowest id
 __device__ __forceinline__ Best best_merge(Best a, Best b) {

@@ -1,8 +1,12 @@
-"""Drafted (speculative) decoding: greedy verification of drafted token trees (include/whisper_amd.h, ``wx_tree_verify``)."""
+"""Drafted (speculative) decoding: greedy verification of drafted token trees (include/whisper_amd.h, ``wx_tree_verify``), where drafts come
+from, and how candidates become a tree.  ``WhisperEngine.decode_draft`` is the loop that uses them.
+
+A drafter is called with the ids of every row so far (prompt included) and the number of ids wanted, and returns for every row a list of
+candidate continuations (lists of ids; none, one or several, of any length)."""
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -49,3 +53,70 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: Optional[to
     a.d_work, a.work_bytes = work.data_ptr(), need
     _check(lib.wx_tree_verify(ref, _raw_stream(dev.index)), "wx_tree_verify")
     return {"pick": pick, "logprob": logprob, "path": path, "n_accept": accept, "next": follow}
+
+
+def draft_tree(last: int, candidates: Sequence[Sequence[int]], max_nodes: int, max_depth: int, stop: int) -> Tuple[List[int], List[int]]:
+    """Candidate continuations as one tree with shared beginnings: (tokens, parents), node 0 is ``last``, the id that is certain.  At most
+    ``max_nodes`` nodes, ``max_depth`` ids below the root; a candidate ends before the id ``stop``.  The candidates grow side by side, id by
+    id, so that a small tree holds the beginning of each."""
+    tokens, parents = [int(last)], [-1]
+    child: Dict[Tuple[int, int], int] = {}
+    at = [0] * len(candidates)
+    alive = list(range(len(candidates)))
+    depth = 0
+    while alive and depth < max_depth:
+        going = []
+        for c in alive:
+            if depth >= len(candidates[c]) or int(candidates[c][depth]) == stop:
+                continue
+            key = (at[c], int(candidates[c][depth]))
+            if key not in child:
+                if len(tokens) >= max_nodes:
+                    continue
+                child[key] = len(tokens)
+                tokens.append(key[1])
+                parents.append(key[0])
+            at[c] = child[key]
+            going.append(c)
+        alive, depth = going, depth + 1
+    return tokens, parents
+
+
+class NgramDraft:
+    """Drafts from the row's own text: what followed the last occurrences of its last ``n`` ids (and, where there is none, of fewer, down
+    to one), the latest first, up to ``branches`` of them.  Costs nothing on the GPU; speech repeats itself, and a prompt holds names."""
+
+    def __init__(self, n: int = 3, branches: int = 2):
+        if n < 1 or branches < 1:
+            raise ValueError("n and branches must be at least 1")
+        self.n, self.branches = int(n), int(branches)
+
+    def __call__(self, rows: Sequence[Sequence[int]], k: int) -> List[List[List[int]]]:
+        out = []
+        for ids in rows:
+            ids, found = list(ids), []
+            for n in range(min(self.n, len(ids) - 1), 0, -1):
+                tail = ids[-n:]
+                for i in range(len(ids) - n - 1, -1, -1):
+                    if ids[i:i + n] == tail:
+                        found.append(ids[i + n:i + n + k])
+                        if len(found) == self.branches:
+                            break
+                if found:
+                    break
+            out.append(found)
+        return out
+
+
+class EngineDraft:
+    """Drafts from another engine with the same vocabulary (a smaller model) that has encoded the same windows: its greedy continuation of
+    every row."""
+
+    def __init__(self, engine):
+        self.engine = engine
+
+    def __call__(self, rows: Sequence[Sequence[int]], k: int) -> List[List[List[int]]]:
+        room = self.engine.dims.n_text_ctx - 1
+        if any(len(r) > room for r in rows):
+            return [[] for _ in rows]
+        return [[t] for t in self.engine.decode_rows(rows, max_new_tokens=k, suppress_blank=False)["tokens"]]

@@ -351,6 +351,136 @@ class WhisperEngine:
         return {"tokens": tokens, "sum_logprobs": sums, "no_speech_probs": nsp.cpu().tolist(), "steps": int(steps.value),
                 "n_prompt": n_prompt, "candidates": cands}
 
+    # -- drafted decoding ---------------------------------------------------------------------------------
+    def draft_cache(self, n_rows: int, n_nodes: int = 64):
+        """A paged cache for ``n_rows`` sequences of this decoder, with room for ``n_nodes`` drafted tokens behind a full context."""
+        from .kvcache import PagedKVCache
+        dims = self.dims
+        if dims.n_text_ctx + n_nodes > 512:
+            raise ValueError(f"n_nodes must be at most {512 - dims.n_text_ctx} (512 tokens a sequence, context included)")
+        pages = -(-(dims.n_text_ctx + n_nodes) // 16)
+        return PagedKVCache.allocate(dims.n_text_layer, dims.n_text_head, 64, n_rows * pages, n_rows, pages, page_size=16,
+                                     dtype=torch.float32 if self.precision == "fp32" else torch.bfloat16, device=self.device)
+
+    def draft_logits(self, cache, seqs: torch.Tensor, tokens: torch.Tensor, parents: Optional[torch.Tensor] = None,
+                     counts: Optional[torch.Tensor] = None, group: int = 1, want_logits: bool = True) -> Optional[torch.Tensor]:
+        """One decoder pass over drafted tokens ``tokens`` [n, n_nodes] of the sequences in cache slots ``seqs`` [n] (int32, on the device;
+        entry i listens to window i // group of the last encode): ``wx_draft_logits``.  Returns the logits [n, n_nodes, n_vocab]."""
+        n, nodes = tokens.shape
+        dev = self.torch_device
+        for t, what, shape in ((seqs, "seqs", (n,)), (tokens, "tokens", (n, nodes)), (parents, "parents", (n, nodes)), (counts, "counts", (n,))):
+            if t is not None and (t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous()):
+                raise ValueError(f"{what} must be a contiguous int32 tensor {list(shape)} on {dev}")
+        stride = int(self.lib.wx_logit_stride(self.handle))
+        logits = torch.empty((n, nodes, stride), dtype=torch.float32, device=dev) if want_logits else None
+        need = int(self.lib.wx_draft_work_bytes(self.handle, n, nodes))
+        _lib.check(min(need, 0), "wx_draft_work_bytes")
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        p = _lib.WxDraftPass(n=n, n_nodes=nodes, group=int(group), want_logits=int(want_logits), d_seqs=seqs.data_ptr(), d_tokens=tokens.data_ptr(),
+                             d_parents=None if parents is None else parents.data_ptr(), d_counts=None if counts is None else counts.data_ptr(),
+                             d_logits=None if logits is None else logits.data_ptr(), d_work=work.data_ptr(), work_bytes=need)
+        _lib.check(self.lib.wx_draft_logits(self.handle, cache._ref, ctypes.byref(p), self._stream()), "wx_draft_logits")
+        return None if logits is None else logits[..., :self.dims.n_vocab]
+
+    def decode_draft(self, prompts: Sequence[Sequence[int]], drafter=None, n_nodes: int = 16, n_draft: int = 8, max_new_tokens: int = 0,
+                     without_timestamps: bool = True, suppress_blank: bool = True) -> Dict[str, object]:
+        """Greedy decode with one prompt per window of the last encode, several ids a pass: ``drafter`` (whisper_amd/draft.py; default
+        ``NgramDraft()``) proposes continuations, one decoder pass answers all of their ids over a paged cache, and the ids that agree with
+        the arg-max are kept.  The ids are greedy's own whatever the drafts (in bf16 up to the rounding of another summation order, as
+        between batch sizes); only the number of passes changes.  ``n_nodes``: most drafted ids of a row in one pass, the certain one
+        included; ``n_draft``: longest continuation asked for.  Timestamp rules depend on the whole row: not offered here.
+
+        Returns ``decode_rows``'s fields, and ``passes`` and ``accepted`` (drafted ids kept)."""
+        from .draft import NgramDraft, draft_tree, verify_tree
+        if not without_timestamps:
+            raise ValueError("decode_draft decodes without timestamps")
+        drafter = NgramDraft() if drafter is None else drafter
+        tok, dims, dev = self.tok, self.dims, self.torch_device
+        rows = [[int(i) for i in p] for p in prompts]
+        n, ctx = len(rows), dims.n_text_ctx
+        if n < 1 or any(not 0 < len(r) < ctx or tok.sot not in r for r in rows) or any(not 0 <= i < dims.n_vocab for r in rows for i in r):
+            raise ValueError("every row needs a prompt of 1 .. n_text_ctx - 1 ids with <|startoftranscript|> in it")
+        if not 1 <= n_nodes <= 64 or n_draft < 1:
+            raise ValueError("n_nodes must be 1 .. 64 and n_draft at least 1")
+        limit = int(max_new_tokens) if max_new_tokens > 0 else ctx // 2
+        cache = self.draft_cache(n, 64)
+        i32 = lambda a: torch.tensor(np.asarray(a, np.int32), device=dev)  # noqa: E731
+        slots = np.arange(n, dtype=np.int32)
+        mask = np.zeros(dims.n_vocab, np.uint8)
+        mask[self.suppress_ids] = 1
+        first = mask.copy()
+        if suppress_blank:
+            first[[tok.blank, tok.eot]] = 1
+        mask, first = torch.from_numpy(mask).to(dev), torch.from_numpy(first).to(dev)
+        # the prompts, all but the last id of each, in chains of up to 64; the no-speech probability at <|startoftranscript|>
+        n_prompt = [len(r) for r in rows]
+        sot = [r.index(tok.sot) for r in rows]
+        no_speech: List[Optional[torch.Tensor]] = [None] * n
+
+        def read_no_speech(logits, base, counts):
+            for b in range(n):
+                if base[b] <= sot[b] < base[b] + counts[b]:
+                    no_speech[b] = torch.softmax(logits[b, sot[b] - base[b]], -1)[tok.no_speech]
+        done = [0] * n
+        while any(done[b] < n_prompt[b] - 1 for b in range(n)):
+            counts = [min(64, n_prompt[b] - 1 - done[b]) for b in range(n)]
+            width = max(counts)
+            ids = np.full((n, width), tok.eot, np.int32)
+            for b in range(n):
+                ids[b, :counts[b]] = rows[b][done[b]:done[b] + counts[b]]
+            seqs, cnt = i32(np.where(np.asarray(counts) > 0, slots, -1)), i32(counts)
+            want = any(done[b] <= sot[b] < done[b] + counts[b] for b in range(n))
+            cache.reserve(seqs, width)
+            logits = self.draft_logits(cache, seqs, i32(ids), counts=cnt, want_logits=want)
+            if want:
+                read_no_speech(logits, done, counts)
+            cache.commit(seqs, torch.arange(width, dtype=torch.int32, device=dev).repeat(n, 1), cnt)
+            done = [done[b] + counts[b] for b in range(n)]
+        sums, live = [0.0] * n, [True] * n
+        passes = accepted = 0
+        begin = True
+        while any(live):
+            trees = [([tok.eot], [-1])] * n
+            # the first id after the prompt has a mask of its own: one node
+            asked = [[] for _ in range(n)] if begin or n_nodes == 1 else drafter(rows, n_draft)
+            for b in range(n):
+                if live[b]:
+                    deep = min(limit - (len(rows[b]) - n_prompt[b]) - 1, ctx - len(rows[b]))      # ids below the root that still count
+                    trees[b] = draft_tree(rows[b][-1], [] if begin else asked[b], n_nodes, max(0, deep), tok.eot)
+            width = max(len(t) for t, _ in trees)
+            ids, par = np.full((n, width), tok.eot, np.int32), np.full((n, width), -1, np.int32)
+            for b, (t, u) in enumerate(trees):
+                ids[b, :len(t)], par[b, :len(u)] = t, u
+            seqs = i32([s if live[s] else -1 for s in slots])
+            d_ids, d_par, counts = i32(ids), i32(par), i32([len(t) for t, _ in trees])
+            cache.reserve(seqs, width)
+            logits = self.draft_logits(cache, seqs, d_ids, d_par, counts)
+            if begin:
+                read_no_speech(logits, [p - 1 for p in n_prompt], [1] * n)
+            r = verify_tree(logits, d_ids, d_par, counts=counts, suppress=first if begin else mask)
+            cache.commit(seqs, r["path"], r["n_accept"])
+            pick, lp, path, taken = (r[k].cpu().numpy() for k in ("pick", "logprob", "path", "n_accept"))
+            begin, passes = False, passes + 1
+            for b in range(n):
+                if not live[b]:
+                    continue
+                for k in range(int(taken[b])):
+                    node = int(path[b, k])
+                    new = int(pick[b, node])
+                    if new < 0:                       # nothing to pick (logits that are no numbers): the row ends, as in the sampler
+                        new, gain = tok.eot, 0.0
+                    else:
+                        gain = float(lp[b, node])
+                    sums[b] += gain
+                    rows[b].append(new)
+                    accepted += k > 0
+                    if new == tok.eot or len(rows[b]) - n_prompt[b] >= limit or len(rows[b]) > ctx:
+                        live[b] = False
+                        break
+        out = [r[p:] for r, p in zip(rows, n_prompt)]
+        return {"tokens": [t[:-1] if t and t[-1] == tok.eot else t for t in out], "sum_logprobs": sums,
+                "no_speech_probs": [0.0 if x is None else float(x) for x in no_speech], "steps": passes, "passes": passes, "accepted": int(accepted)}
+
     def last_profile(self):
         """(total_ms, launches) of the cross-attention launches bracketed by the last profiled eager decode."""
         ms, n = ctypes.c_double(0.0), ctypes.c_int64(0)
@@ -390,9 +520,17 @@ class WhisperEngine:
         return seq
 
     def transcribe_mel(self, mel: torch.Tensor, n_content_frames: int, window_lo: int, window_hi: int,
-                       prompt: Sequence[int], beam_size: Optional[int] = None, patience: float = 1.0, **decode_kw) -> Dict[str, object]:
+                       prompt: Sequence[int], beam_size: Optional[int] = None, patience: float = 1.0, draft=None, **decode_kw) -> Dict[str, object]:
         """Decode windows [window_lo, window_hi) of a whole-file mel ``[n_mels, ld]`` in batches of ``max_batch`` windows
-        (greedy) or ``max_batch // beam_size`` windows (beam search: rows = windows x beams)."""
+        (greedy) or ``max_batch // beam_size`` windows (beam search: rows = windows x beams).  ``draft``: greedy by ``decode_draft`` with
+        this drafter ("ngram": ``NgramDraft()``)."""
+        if draft is not None and beam_size:
+            raise ValueError("draft and beam_size exclude each other")
+        if isinstance(draft, str):
+            if draft != "ngram":
+                raise ValueError("draft must be 'ngram' or a drafter (whisper_amd/draft.py)")
+            from .draft import NgramDraft
+            draft = NgramDraft()
         toks: List[List[int]] = []
         sums: List[float] = []
         nsp: List[float] = []
@@ -407,6 +545,9 @@ class WhisperEngine:
             self.encode(view, N_FRAMES, ld, n_content_frames - w0 * N_FRAMES, B)
             if beam_size:
                 r = self.decode_beam(B, prompt, beam_size=int(beam_size), patience=patience, **decode_kw)
+                toks += r["tokens"]; sums += r["sum_logprobs"]; nsp += r["no_speech_probs"]
+            elif draft is not None:
+                r = self.decode_draft([list(prompt)] * B, draft, **decode_kw)
                 toks += r["tokens"]; sums += r["sum_logprobs"]; nsp += r["no_speech_probs"]
             else:
                 r = self.decode_greedy(B, prompt, **decode_kw)
