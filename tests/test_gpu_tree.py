@@ -227,6 +227,33 @@ def test_other_stream_and_replayed_graph():
         assert torch.equal(out, eager)
 
 
+def test_offsets_past_32_bits():
+    """the last layer and the last pages of pools of 9 GB: the same results as in a small pool, and pages copied, appended to and moved there"""
+    H, D, PS, L, P = 8, 128, 64, 3, 24000
+    big = PagedKVCache.allocate(L, H, D, P, 3, 20, page_size=PS, dtype=BF16)
+    small = PagedKVCache.allocate(1, H, D, 8, 3, 20, page_size=PS, dtype=BF16)
+    assert big.k.numel() > 2 ** 32
+    big.refs.fill_(1)
+    big.refs[P - 8:] = 0
+    ids = i32([0])
+    kv = torch.randn(2, 1, 1, 200, H, D, device="cuda").to(BF16)
+    q = torch.randn(1, 1, 4 * H, D, device="cuda").to(BF16)
+    outs = []
+    for cache, layer in ((big, 2), (small, 0)):
+        assert cache.reserve(ids, 200).tolist() == [0]
+        cache.append(ids, kv[0, 0], kv[1, 0], layer=layer)
+        cache.commit(ids, i32([list(range(0, 150)) + [199] + [-1] * 49]), i32([151]))
+        assert cache.fork(i32([1]), ids).tolist() == [0] and cache.reserve(i32([1]), 5).tolist() == [0]
+        new = kv[:, 0, :, 7:12]
+        outs.append(cache.attend(layer, i32([1]), q.expand(1, 5, 4 * H, D), k=new[0], v=new[1]))
+    assert big.table[1, 0] >= P - 8 and torch.equal(outs[0], outs[1])
+    for t in (0, 1):
+        rows = int(small.lens[t].item())
+        for pos in (0, 63, 64, 150, rows - 1):
+            a = big.k[2, int(big.table[t, pos // PS]), :, pos % PS]
+            assert torch.equal(a, small.k[0, int(small.table[t, pos // PS]), :, pos % PS])
+
+
 def test_attend_refusals():
     c = Case([4], 2, 2, 2, 64, 16, BF16)
     s = i32(c.slots)

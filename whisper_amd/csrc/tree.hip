@@ -1200,8 +1200,7 @@ __global__ __launch_bounds__(VF_NT) void tree_verify_scan_kernel(wx_tree_check a
     __syncthreads();
     if (tid == 0) {
         for (int w = 1; w < VF_NT / 64; ++w) b = best_merge(b, sh[w]);
-        float* rec = reinterpret_cast<float*>(a.d_work) + (((int64_t)i * a.n_nodes + node) * parts + part) * 4;
-        rec[0] = b.m; rec[1] = b.s; reinterpret_cast<int*>(rec)[2] = b.i;
+        reinterpret_cast<f32x4*>(a.d_work)[((int64_t)i * a.n_nodes + node) * parts + part] = f32x4{b.m, b.s, __builtin_bit_cast(float, b.i), 0.f};
     }
 }
 
@@ -1213,8 +1212,9 @@ __global__ __launch_bounds__(64) void tree_verify_walk_kernel(wx_tree_check a, i
     float lp = 0.f;
     if (j < count) {
         Best b{-INFINITY, 0.f, 0x7fffffff};
-        const float* rec = reinterpret_cast<const float*>(a.d_work) + ((int64_t)i * a.n_nodes + j) * parts * 4;
-        for (int p = 0; p < parts; ++p) b = best_merge(b, Best{rec[4 * p], rec[4 * p + 1], reinterpret_cast<const int*>(rec)[4 * p + 2]});
+        const f32x4* rec = reinterpret_cast<const f32x4*>(a.d_work) + ((int64_t)i * a.n_nodes + j) * parts;
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) { const f32x4 x = rec[p]; b = best_merge(b, Best{x[0], x[1], __builtin_bit_cast(int, (float)x[2])}); }
         pick = b.m > -INFINITY ? b.i : -1;
         lp = b.m > -INFINITY ? -logf(b.s) : -INFINITY;
         token = a.d_tokens[(int64_t)i * a.n_nodes + j];
@@ -1289,7 +1289,7 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
     const int64_t need = tree_part_bytes(*c, p);
     if (need > 0 && (!a->d_work || a->work_bytes < need || ((uintptr_t)a->d_work & 15))) return set_error(WX_ERR_INVALID, "work buffer too small or not 16-byte aligned");
     const int64_t jobs = ((int64_t)p.slots * c->n_kv_head + 7) / 8 * 8 * p.row_blocks;
-    if (jobs > 0x7fffffff) return set_error(WX_ERR_INVALID, "too many pieces: larger split_tokens, or fewer sequences");
+    if (jobs > 0x7fffff) return set_error(WX_ERR_INVALID, "too many pieces of work: fewer sequences, or larger split_tokens");
     const dim3 grid((unsigned)jobs), block(256);
     const bool f32 = c->precision == WX_PREC_F32, wide = c->head_dim == 128;
 #define TREE_KEYS(T, D, RT) do { if (p.single) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, true>), grid, block, 0, st, TreeArgs{*c, *a, p}); \

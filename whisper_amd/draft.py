@@ -38,21 +38,25 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: Optional[to
         if not torch.is_tensor(t) or t.dtype != dtype or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
             raise ValueError(f"{what} must be a contiguous {dtype} tensor {list(shape)} on {dev}")
     lib = _lib.load()
-    i32 = dict(dtype=torch.int32, device=dev)
-    pick, path, accept, follow = torch.empty((n, nodes), **i32), torch.empty((n, nodes), **i32), torch.empty(n, **i32), torch.empty(n, **i32)
-    logprob = torch.empty((n, nodes), dtype=torch.float32, device=dev)
+    # one allocation for the whole numbers (each tensor is a host call), one for the log-probabilities
+    cells = n * nodes
     a = _lib.WxTreeCheck(n, nodes, vocab, _PRECISION[logits.dtype], dev.index, logits.data_ptr(), logits.stride(0), logits.stride(1), tokens.data_ptr(),
                          None if parents is None else parents.data_ptr(), None if counts is None else counts.data_ptr(),
-                         None if suppress is None else suppress.data_ptr(), pick.data_ptr(), logprob.data_ptr(), path.data_ptr(), accept.data_ptr(),
-                         follow.data_ptr())
+                         None if suppress is None else suppress.data_ptr())
     ref = ctypes.byref(a)
     need = lib.wx_tree_verify_work_bytes(ref)
     if need < 0:
         _check(int(need), "wx_tree_verify")
-    work = torch.empty(need, dtype=torch.uint8, device=dev)
-    a.d_work, a.work_bytes = work.data_ptr(), need
+    buf = torch.empty(need // 4 + 2 * cells + 2 * n, dtype=torch.int32, device=dev)
+    logprob = torch.empty((n, nodes), dtype=torch.float32, device=dev)
+    _, pick, path, accept, follow = buf.split_with_sizes((need // 4, cells, cells, n, n))
+    base = buf.data_ptr()
+    a.d_work, a.work_bytes = base, need
+    a.d_pick, a.d_path = base + need, base + need + 4 * cells
+    a.d_n_accept, a.d_next = base + need + 8 * cells, base + need + 8 * cells + 4 * n
+    a.d_logprob = logprob.data_ptr()
     _check(lib.wx_tree_verify(ref, _raw_stream(dev.index)), "wx_tree_verify")
-    return {"pick": pick, "logprob": logprob, "path": path, "n_accept": accept, "next": follow}
+    return {"pick": pick.view(n, nodes), "logprob": logprob, "path": path.view(n, nodes), "n_accept": accept, "next": follow}
 
 
 def draft_tree(last: int, candidates: Sequence[Sequence[int]], max_nodes: int, max_depth: int, stop: int) -> Tuple[List[int], List[int]]:

@@ -135,7 +135,8 @@ def transcribe(audio, language: Optional[str] = None, prompt: Union[None, str, S
     itself; the result additionally carries ``segments``.
 
     ``decode_kw``: ``beam_size`` (None = greedy, upstream's default for the reference's call), ``patience``,
-    ``max_new_tokens``, ``without_timestamps``.
+    ``max_new_tokens``, ``without_timestamps``, ``draft`` (windows mode, greedy: several ids a decoder pass, "ngram" or a drafter of
+    whisper_amd/draft.py).
 
     Returns ``{"text", "confidence", "chunks_processed"}`` plus ``language``, ``tokens`` (per window),
     ``avg_logprob`` and ``no_speech_prob`` (per window).
@@ -153,6 +154,8 @@ def transcribe(audio, language: Optional[str] = None, prompt: Union[None, str, S
     cmode = (_STATE["settings"] or {}).get("confidence_mode", "reference")
     lang_idx = None if language is None else language_index(language, eng.dims.n_vocab)
     if mode == "sequential":
+        if "draft" in decode_kw:
+            raise ValueError("draft needs mode='windows' (the sequential loop decodes with timestamps)")
         from .longform import transcribe_sequential
         r = transcribe_sequential(eng, [pcm_host], tokenizer.decode, language_index=lang_idx,
                                   initial_prompts=[_prompt_ids(prompt, tokenizer)], **decode_kw)[0]
