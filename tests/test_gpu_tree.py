@@ -103,6 +103,17 @@ def test_against_64_bits(dtype, lens, N, heads, kv_heads, D, PS, append):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("n,N,heads,kv_heads,D,longest", [(1, 3, 1, 1, 64, 5000), (3, 2, 2, 1, 128, 3000), (8, 64, 8, 4, 64, 700), (17, 64, 8, 4, 64, 640), (33, 64, 8, 8, 64, 560),
+                                                          (9, 33, 8, 4, 128, 700), (24, 33, 16, 8, 128, 530)])
+def test_many_pieces_and_many_rows(dtype, n, N, heads, kv_heads, D, longest):
+    """a merge with one row a workgroup (all threads on its pieces), with some, and with as many as it holds"""
+    lens = np.random.RandomState(n).randint(0, longest + 1, n)
+    lens[-1] = longest
+    c = Case(lens, N, heads, kv_heads, D, 16, dtype, seed=n)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
 def test_ragged_counts_padding_and_chain(dtype):
     c = Case([40, 3, 0, 100], 12, 4, 2, 64, 16, dtype, counts=[12, 0, 5, 1])
     c.check(c.run())

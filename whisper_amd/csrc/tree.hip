@@ -14,18 +14,19 @@ constexpr float TR_LOG2E = 1.4426950408889634f;
 
 // How the work on a batch is cut.  A sequence has ceil(len / KT) tiles of committed tokens and `tree_tiles` behind them.  For every
 // key / value head and block of rows, `takers` workgroups take equal shares of all sequences' tiles in a row (fewer takers where a
-// share would fall below `least` tiles), so that ragged lengths leave no workgroup behind: one may end a sequence, do some whole ones
-// and begin another.  The part of a sequence that taker w does is piece w + i of the part buffer (w or i grows by one from piece to
-// piece, so the numbers are distinct).  With `per` > 0 a sequence is cut into pieces of at most `per` tiles instead, one for each
-// workgroup; with `single`, where no sequence can be longer than `least` tiles, a workgroup does one whole sequence.
+// share would fall below `least` tiles, or `least_few` with up to `few` takers), so that ragged lengths leave no workgroup behind: one may
+// end a sequence, do some whole ones and begin another.  The part of a sequence that taker w does is piece w + i of the part buffer (w or i
+// grows by one from piece to piece, so the numbers are distinct).  With `per` > 0 a sequence is cut into pieces of at most `per` tiles instead, one for each
+// workgroup; with `single`, where no sequence can be longer than 512 tokens, a workgroup does one whole sequence.
 struct TreePlan {
     int row_blocks;          // workgroups over the rows (nodes x query heads of a key / value head)
-    int tree_tiles, per, least, takers;
+    int tree_tiles, per, least, takers, least_few, few;
     int single;              // (the kernels' ONE)
     int shift;               // log2 of the page size
     int slots;               // workgroups for each key / value head and block of rows
     int pieces;              // ... and places for their parts
     int rows;                // rows a workgroup
+    int merge_rows;          // rows a workgroup of the merge (a power of two); the rest of its threads share their pieces
     float* part;             // [pieces][n_kv_head][row_blocks][rows][D + 2]: output, maximum and sum (sequences in more than one piece)
 };
 
@@ -43,7 +44,7 @@ __device__ __forceinline__ int64_t tree_all(const wx_cache& c, const wx_tree_att
     for (int i = lane; i < a.n; i += 64) all += tree_tiles_of(c, a, p, i, kt);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
-    *takers = (int)max((int64_t)1, min((int64_t)p.takers, all / p.least));
+    *takers = (int)max((int64_t)1, min((int64_t)p.takers, max(all / p.least, min((int64_t)p.few, all / p.least_few))));
     return all;
 }
 
@@ -997,15 +998,16 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G;
     const float cc = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * TR_LOG2E;
     constexpr int TPR = D / 4, RPB = 256 / TPR;
-    const int row = blockIdx.z * RPB + tid / TPR, x = (tid % TPR) * 4;
-    if (row >= rows) return;
-    const int node = row / G;
+    __shared__ f32x4 s_v[RPB][TPR];
+    __shared__ float s_m[RPB], s_l[RPB];
+    const int slot = tid / TPR, groups = RPB / p.merge_rows, group = slot / p.merge_rows;
+    const int row = blockIdx.z * p.merge_rows + slot % p.merge_rows, x = (tid % TPR) * 4;
     const int64_t step = (int64_t)c.n_kv_head * p.row_blocks * p.rows * (D + 2);
-    const float* part = p.part + ((((int64_t)first * c.n_kv_head + kh) * p.row_blocks + row / p.rows) * p.rows + row % p.rows) * (D + 2);
+    const float* part = p.part + ((((int64_t)first * c.n_kv_head + kh) * p.row_blocks + min(row, rows - 1) / p.rows) * p.rows + min(row, rows - 1) % p.rows) * (D + 2);
     // four pieces' loads at a time, one running maximum (a launch of this size is bound by the loads' latency)
     float M = -INFINITY, L = 0.f;
     f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int q0 = 0; q0 < pieces; q0 += 4) {
+    for (int q0 = 4 * group; q0 < pieces; q0 += 4 * groups) {
         float m[4], l[4];
         f32x2 lo[4], hi[4];
 #pragma unroll
@@ -1028,6 +1030,21 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
                 v += f32x4{lo[q][0], lo[q][1], hi[q][0], hi[q][1]} * f;
             }
     }
+    if (groups > 1) {                                                               // the groups' parts, in order
+        s_v[slot][tid % TPR] = v;
+        if (x == 0) { s_m[slot] = M; s_l[slot] = L; }
+        __syncthreads();
+        if (group > 0) return;
+        for (int o = slot + p.merge_rows; o < RPB; o += p.merge_rows) {
+            const float mo = s_m[o], mn = fmaxf(M, mo);
+            const float fa = M == mn ? 1.f : __builtin_amdgcn_exp2f((M - mn) * cc), fb = mo == mn ? 1.f : __builtin_amdgcn_exp2f((mo - mn) * cc);
+            M = mn;
+            L = L * fa + s_l[o] * fb;
+            v = v * fa + s_v[o][tid % TPR] * fb;
+        }
+    }
+    if (row >= rows) return;
+    const int node = row / G;
     T* out = reinterpret_cast<T*>(a.d_out) + i * a.o_seq + node * a.o_node + (kh * G + row % G) * a.o_head + x;
     const int kind = seq == -1 || node >= count ? 0 : s_wrong[node] ? 2 : 1;
     store4<T>(out, kind == 1 ? v * (1.f / L) : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
@@ -1072,15 +1089,25 @@ static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeFo
     while ((1 << p.shift) < c.page_size) ++p.shift;
     const int64_t most = ((int64_t)c.max_pages * c.page_size + f.kt - 1) / f.kt + p.tree_tiles;       // tiles of the longest sequence the tables hold
     const int64_t units = (int64_t)c.n_kv_head * p.row_blocks;
+    // Shares of 512 tokens at least, but of 128 up to the first 256 workgroups, which leave compute units idle: one sequence of 40575 tokens,
+    // 1 head of 64, f32: 37 us with 512, 23 with 128, 25 with 64; 7 sequences of up to 1912, 1 head of 128, f32: 39, 28, 26; 5 of up to 2283,
+    // 20 heads of 128, bf16 (260 shares of 512): 28, 36.  Tables of up to 512 tokens are not cut at all: the second launch costs 5 us and the
+    // pieces save less (1 x 430 tokens, 20 heads of 64: 12 us whole, 18 cut).
     p.least = 512 / f.kt + p.tree_tiles;
+    p.least_few = 128 / f.kt + p.tree_tiles;
+    p.few = (int)((255 + units) / units);
     p.takers = (int)(((f.rows_form ? 256 : 768) + units - 1) / units);
     if (a.split_tokens > 0) {                                                       // at most 256 pieces a sequence
         p.per = (int)(((int64_t)a.split_tokens + f.kt - 1) / f.kt);
         if (p.per < (most + 255) / 256) p.per = (int)((most + 255) / 256);
     }
-    p.single = most <= (p.per ? p.per : p.least);
+    p.single = most <= (p.per ? p.per : 512 / f.kt + p.tree_tiles);
     p.slots = p.single ? a.n : p.per ? (int)(a.n * ((most + p.per - 1) / p.per)) : p.takers;
     p.pieces = p.single ? 0 : p.per ? p.slots : p.takers + a.n;
+    // the merge: as few rows a workgroup (as many threads on a row's pieces) as leave it at most 2048 workgroups (6 sequences of up to 38255
+    // tokens, 2 heads of 64, f32, shares of 128: 55 us so, 67 with every row's pieces on one group of threads)
+    p.merge_rows = 1024 / c.head_dim;
+    while (p.merge_rows > 1 && units * a.n * ((rows + p.merge_rows / 2 - 1) / (p.merge_rows / 2)) <= 2048 * (int64_t)p.row_blocks) p.merge_rows /= 2;
     return p;
 }
 static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {
@@ -1308,8 +1335,8 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
         else { if (f.rt == 2) TREE_KEYS(bf16, 64, 2); else TREE_KEYS(bf16, 64, 1); }
     }
     if (!p.single) {
-        const int rows = a->n_nodes * (a->n_head / c->n_kv_head), rpb = 1024 / c->head_dim;
-        const dim3 mg(a->n, c->n_kv_head, (rows + rpb - 1) / rpb);
+        const int rows = a->n_nodes * (a->n_head / c->n_kv_head);
+        const dim3 mg(a->n, c->n_kv_head, (rows + p.merge_rows - 1) / p.merge_rows);
         if (f32) {
             if (wide) hipLaunchKernelGGL((tree_attention_merge_kernel<float, 128, 16>), mg, block, 0, st, *c, *a, p);
             else hipLaunchKernelGGL((tree_attention_merge_kernel<float, 64, 32>), mg, block, 0, st, *c, *a, p);
