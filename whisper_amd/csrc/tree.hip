@@ -1095,8 +1095,14 @@ static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeFo
     // pieces save less (1 x 430 tokens, 20 heads of 64: 12 us whole, 18 cut).
     p.least = 512 / f.kt + p.tree_tiles;
     p.least_few = 128 / f.kt + p.tree_tiles;
-    p.few = (int)((255 + units) / units);
-    p.takers = (int)(((f.rows_form ? 256 : 768) + units - 1) / units);
+    p.few = (int)(units < 256 ? 256 / units : 1);
+    // As many workgroups as run at once (one a compute unit that shares rows, two that share keys), never a few more, which would run alone at
+    // the end: 3 sequences of up to 32792 tokens, 12 heads, 184 rows: 264 workgroups 240 us, 252 148 us; 16 x 24 rows, 20 heads of 64, 4000-16000
+    // tokens: 512 workgroups 182 us, 768 203 us.  Where heads and row blocks do not divide that number nearly, four times as many smaller ones.
+    const int64_t slots = f.rows_form ? 256 : 512;
+    int64_t takers = slots / units;
+    if (5 * takers * units < 4 * slots) takers = 4 * slots / units;
+    p.takers = (int)(takers > 1 ? takers : 1);
     if (a.split_tokens > 0) {                                                       // at most 256 pieces a sequence
         p.per = (int)(((int64_t)a.split_tokens + f.kt - 1) / f.kt);
         if (p.per < (most + 255) / 256) p.per = (int)((most + 255) / 256);
