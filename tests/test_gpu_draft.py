@@ -142,6 +142,45 @@ def test_node_logits_against_the_decoder(precision, max_batch, monkeypatch):
         eng.close()
 
 
+@pytest.mark.parametrize("group,N", [(1, 1), (1, 2), (1, 8), (1, 9), (1, 40), (2, 21), (3, 53), (3, 54)])
+@pytest.mark.parametrize("windows", [1, 2])
+def test_every_size_of_pass(group, N, windows):
+    """chains of every number of rows a pass treats differently, against the decoder's logits position by position, the second half of the
+    rows behind a committed first half.
+
+    fp32: the bar of the engine's own logit tests.  bf16: this network of random weights amplifies a rounding, so the bar is its own: the
+    decoder's distance from the fp32 engine's logits.  That distance comes from half a step of 2^-8 in every weight and in every stored
+    activation, two kinds at each of ten products a layer.  Pass and decoder share the weights; they round differently at three places a
+    layer (the probabilities of both attentions, and sums of another order), on two sides: sqrt(2 x 3 / 20) = 0.55 of it if errors add up
+    as a random walk does.  Half of it is asked for; a row that met a wrong row, weight or window is off by about the logits' size."""
+    dist = lambda a, b: float(((a - b).abs().amax(-1) / b.abs().amax(-1)).max())  # noqa: E731
+    n, rng = windows * group, np.random.RandomState(N)
+    tok = rng.randint(0, 300, (n, 2 * N)).astype(np.int32)
+    seen = {}
+    for precision in ("fp32", "bf16"):
+        eng, _, _ = make(precision, 2, name="tiny", windows=windows)
+        try:
+            assert eng.cross_form == "kv"
+            cache = eng.draft_cache(n)
+            slots = torch.arange(n, dtype=torch.int32, device="cuda")
+            d = torch.from_numpy(tok).cuda()
+            got = []
+            for half in (0, 1):
+                cache.reserve(slots, N)
+                got.append(eng.draft_logits(cache, slots, d[:, half * N:half * N + N].contiguous(), group=group))
+                path = torch.arange(N, dtype=torch.int32, device="cuda").repeat(n, 1)
+                assert not cache.commit(slots, path, torch.full((n,), N, dtype=torch.int32, device="cuda")).any()
+            got = torch.cat(got, 1).cpu()
+            want = torch.empty_like(got)
+            for k in range(group):                                   # entry k of every window's group
+                want[k::group] = eng.decoder_logits(torch.from_numpy(tok[k::group].copy())).cpu()[..., :got.shape[-1]]
+            seen[precision] = got, want
+        finally:
+            eng.close()
+    assert dist(*seen["fp32"]) < 1e-4
+    assert dist(*seen["bf16"]) <= 0.5 * dist(seen["bf16"][1], seen["fp32"][1])
+
+
 def test_windows_path_with_ngram_drafts():
     eng, mel, _ = make(max_batch=2, windows=3)
     try:

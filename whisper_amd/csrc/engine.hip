@@ -1467,13 +1467,17 @@ int wx_decoder_logits(wx_engine* e, int32_t B, const int32_t* d_tokens, int32_t 
 }
 
 // ---- drafted decoding on the caller's cache (include/whisper_amd.h: wx_draft_logits) -----------------------------------------------------
-// The decoder layers as decode_step_f32 has them (every GEMM applies its own epilogue), for n x n_nodes rows: self-attention is the tree
-// attention over the cache (which appends the rows' keys and values), cross-attention the encoder's kernels on the cached K/V, the rows
-// of a window being its queries.
+// The decoder layers for n x n_nodes rows: self-attention is the tree attention over the cache (which appends the rows' keys and values),
+// cross-attention runs on the cached K/V, the rows of a window being its queries.  bf16 rows up to DRAFT_SPLIT_ROWS take the decode
+// path's GEMMs, as many rows at a time as those take (later rows find the weights in the Infinity Cache): residual products split K and hand
+// their 32-bit tiles to the next LayerNorm, the others halve K inside the workgroup.  More rows, and fp32, take the general GEMMs, which
+// apply their own epilogues.  A pass of large-v3 in bf16 at 1 x 8 nodes: 2.2 ms, 6.4 on the general GEMMs (a step of one token: 1.5); at
+// 32 x 8 nodes: 9.3 against 11.2.
+constexpr int DRAFT_SPLIT_ROWS = 320, DRAFT_CROSS_SPLIT = 6;
 }  // extern "C"
 
 static size_t draft_round(size_t b) { return (b + 255) & ~(size_t)255; }
-struct DraftWork { float* x; char *xn, *qkv, *att, *hid, *q; size_t bytes; };
+struct DraftWork { float* x; char *xn, *qkv, *att, *hid, *q; float *tiles, *parts; size_t bytes; };
 static DraftWork draft_work(const wx_engine* e, int64_t rows, char* base) {
     const size_t es = dtype_size(e->dt), d = e->d;
     DraftWork w;
@@ -1481,6 +1485,11 @@ static DraftWork draft_work(const wx_engine* e, int64_t rows, char* base) {
     auto take = [&](size_t bytes) { char* p = base + at; at += draft_round(bytes); return p; };
     w.x = (float*)take(rows * d * 4);
     w.xn = take(rows * d * es); w.qkv = take(rows * 3 * d * es); w.att = take(rows * d * es); w.hid = take(rows * 4 * d * es); w.q = take(rows * d * es);
+    w.tiles = w.parts = nullptr;
+    if (e->dt == DT_BF16 && rows <= DRAFT_SPLIT_ROWS) {
+        w.tiles = (float*)take((size_t)16 * (rows < DG_MAX_ROWS ? rows : DG_MAX_ROWS) * d * 4);
+        w.parts = (float*)take(rows * e->Ht * DRAFT_CROSS_SPLIT * (HEAD_DIM + 2) * 4);
+    }
     w.bytes = at;
     return w;
 }
@@ -1515,20 +1524,49 @@ int wx_draft_logits(wx_engine* e, const wx_cache* c, const wx_draft_pass* p, voi
     const DraftWork w = draft_work(e, R, (char*)p->d_work);
     const size_t cross_layer = (size_t)k.max_batch * e->Ht * T * HEAD_DIM;
     WX_TRY(launch_tree_embed(e->tok_emb, e->dec_pos, dtp, *c, p->d_seqs, p->d_tokens, p->d_parents, p->n, p->n_nodes, w.x, d, st, k.n_vocab, k.n_text_ctx));
+    const bool few = w.tiles != nullptr;
+    const int passes = (R + DG_MAX_ROWS - 1) / DG_MAX_ROWS, step = few ? ((R + passes - 1) / passes + 15) / 16 * 16 : R;
+    const int s_dd = decode_gemm_split(d, d), s_fc2 = decode_gemm_split(d, 4 * d);
+    // out = epilogue(A W^T + bias)
+    auto product = [&](const char* A, int K, const void* W, const void* Wpk, const float* bias, int N, char* out, int act, int scaled) {
+        for (int r0 = 0; r0 < R; r0 += step) {
+            GemmArgs g = gemm_basic(e, A + (size_t)r0 * K * es, K, W, R - r0 < step ? R - r0 : step, N, K);
+            g.ep.bias = bias; g.ep.act = act; g.ep.out = out + (size_t)r0 * N * es; g.ep.out_dtype = dtp; g.ep.ldo = N;
+            if (scaled) { g.ep.colscale_period = d; for (int t = 0; t < scaled; ++t) g.ep.colscale[t] = e->qk_scale; }
+            if (few) g.Wpk = Wpk;
+            int r = few && Wpk ? launch_gemm_khalf(g, st) : 1;
+            if (r == 1) r = launch_gemm(g, st);
+            if (r) return r;
+        }
+        return 0;
+    };
+    // x += A W^T + bias, xn = LayerNorm(x)
+    auto residual = [&](const char* A, int K, const void* W, const void* Wpk, const float* bias, int split, const float* gamma, const float* beta) {
+        for (int r0 = 0; r0 < R; r0 += step) {
+            const int rows = R - r0 < step ? R - r0 : step;
+            GemmArgs g = gemm_basic(e, A + (size_t)r0 * K * es, K, W, rows, d, K);
+            float* x = w.x + (size_t)r0 * d;
+            char* xn = w.xn + (size_t)r0 * d * es;
+            int r;
+            if (few) {
+                g.Wpk = Wpk; g.n_split = split; g.partial = w.tiles;
+                if (split == 1) { g.ep.out = w.tiles; g.ep.out_dtype = DT_F32; g.ep.ldo = d; }
+                r = launch_gemm(g, st);
+                if (!r) r = launch_reduce_layernorm(x, w.tiles, split, bias, gamma, beta, xn, dtp, rows, d, st);
+            } else {
+                g.ep.bias = bias; g.ep.out = x; g.ep.out_dtype = DT_F32; g.ep.ldo = d; g.ep.residual = x; g.ep.ldr = d;
+                r = launch_gemm(g, st);
+                if (!r) r = launch_layernorm(x, gamma, beta, xn, dtp, rows, d, st);
+            }
+            if (r) return r;
+        }
+        return 0;
+    };
+    WX_TRY(launch_layernorm(w.x, e->dec[0].ln1_g, e->dec[0].ln1_b, w.xn, dtp, R, d, st));
     for (int i = 0; i < k.n_text_layer; ++i) {
         const LayerW& L = e->dec[i];
-        auto gemm = [&](const void* A, int64_t lda, const void* W, int N, int K, const float* bias, void* out, int out_dt, int64_t ldo) {
-            GemmArgs g = gemm_basic(e, A, lda, W, R, N, K);
-            g.ep.bias = bias; g.ep.out = out; g.ep.out_dtype = out_dt; g.ep.ldo = ldo;
-            return g;
-        };
-        auto residual = [&](GemmArgs g) { g.ep.residual = w.x; g.ep.ldr = d; return launch_gemm(g, st); };
-        WX_TRY(launch_layernorm(w.x, L.ln1_g, L.ln1_b, w.xn, dtp, R, d, st));
-        {
-            GemmArgs g = gemm(w.xn, d, L.self.wqkv, 3 * d, d, L.self.bqkv, w.qkv, dtp, 3 * d);
-            g.ep.colscale_period = d; g.ep.colscale[0] = e->qk_scale; g.ep.colscale[1] = e->qk_scale;
-            WX_TRY(launch_gemm(g, st));
-        }
+        const bool last = i + 1 == k.n_text_layer;
+        WX_TRY(product(w.xn, d, L.self.wqkv, L.self.wqkv_pk, L.self.bqkv, 3 * d, w.qkv, 0, 2));
         {
             wx_tree_attn a{};
             a.layer = i; a.n = p->n; a.n_nodes = p->n_nodes; a.n_head = e->Ht;
@@ -1540,31 +1578,36 @@ int wx_draft_logits(wx_engine* e, const wx_cache* c, const wx_draft_pass* p, voi
             a.scale = 1.f;                                                    // q and k carry head_dim^-0.25 each
             if (int r = wx_tree_attention(c, &a, stream)) return r;
         }
-        WX_TRY(residual(gemm(w.att, d, L.self.wo, d, d, L.self.bo, w.x, DT_F32, d)));
-        WX_TRY(launch_layernorm(w.x, L.lnx_g, L.lnx_b, w.xn, dtp, R, d, st));
-        {
-            GemmArgs g = gemm(w.xn, d, L.xq, d, d, L.xbq, w.q, dtp, d);
-            g.ep.colscale_period = d; g.ep.colscale[0] = e->qk_scale;
-            WX_TRY(launch_gemm(g, st));
-        }
+        if (last && !p->want_logits) return WX_OK;                            // the cache has all rows: nothing else was asked for
+        WX_TRY(residual(w.att, d, L.self.wo, L.self.wo_pk, L.self.bo, s_dd, L.lnx_g, L.lnx_b));
+        WX_TRY(product(w.xn, d, L.xq, L.xq_pk, L.xbq, d, w.q, 0, 1));
         {
             AttnArgs a;
-            a.dt = dtp; a.Q = w.q; a.q_sb = (int64_t)per_window * d; a.q_sq = d; a.q_sh = HEAD_DIM; a.n_q = per_window;
+            a.dt = dtp; a.Q = w.q; a.O = w.att; a.H = e->Ht; a.q_sh = a.o_sh = HEAD_DIM;
             a.K = (char*)e->crossK + cross_layer * i * es; a.V = (char*)e->crossV + cross_layer * i * es; a.kv_sbh = (int64_t)T * HEAD_DIM; a.n_keys = T;
-            a.O = w.att; a.o_sb = (int64_t)per_window * d; a.o_sq = d; a.o_sh = HEAD_DIM; a.B = windows; a.H = e->Ht;
-            WX_TRY(dtp == DT_BF16 ? launch_attn_flash_bf16(a, st) : launch_attn_rows(a, st));
+            // Few rows share a window's stream in the single-token kernel (vector pipe, cut along the keys), eight at a time; more take the encoder's
+            // kernel (matrix pipe, one workgroup a window and head: one window's 1500 keys last 35 us whatever the rows).  A pass of large-v3:
+            // 1 x 8 nodes 2.2 against 3.3 ms, 4 x 8 the same, 8 x 8 4.3 against 3.5; 32 x 2 3.7 against 4.2.
+            if (few && (per_window <= 2 || (R <= 16 && (per_window <= 8 || windows == 1)))) {
+                a.q_sb = a.o_sb = d; a.n_q = 1; a.partial = w.parts;
+                a.n_split = 1;
+                while (a.n_split < DRAFT_CROSS_SPLIT && k.max_batch * e->Ht * a.n_split < 512) ++a.n_split;
+                const int most = windows == 1 ? 8 : R;
+                for (int r0 = 0; r0 < R; r0 += most) {
+                    a.Q = w.q + (size_t)r0 * d * es; a.O = w.att + (size_t)r0 * d * es;
+                    a.B = R - r0 < most ? R - r0 : most;
+                    a.kv_group = windows == 1 ? a.B : per_window;
+                    WX_TRY(launch_attn_decode(a, st));
+                }
+            } else {
+                a.q_sb = a.o_sb = (int64_t)per_window * d; a.q_sq = a.o_sq = d; a.n_q = per_window; a.B = windows;
+                WX_TRY(dtp == DT_BF16 ? launch_attn_flash_bf16(a, st) : launch_attn_rows(a, st));
+            }
         }
-        WX_TRY(residual(gemm(w.att, d, L.xo, d, d, L.xbo, w.x, DT_F32, d)));
-        WX_TRY(launch_layernorm(w.x, L.ln2_g, L.ln2_b, w.xn, dtp, R, d, st));
-        {
-            GemmArgs g = gemm(w.xn, d, L.w1, 4 * d, d, L.b1, w.hid, dtp, 4 * d);
-            g.ep.act = 1;
-            WX_TRY(launch_gemm(g, st));
-        }
-        WX_TRY(residual(gemm(w.hid, 4 * d, L.w2, d, 4 * d, L.b2, w.x, DT_F32, d)));
+        WX_TRY(residual(w.att, d, L.xo, L.xo_pk, L.xbo, s_dd, L.ln2_g, L.ln2_b));
+        WX_TRY(product(w.xn, d, L.w1, L.w1_pk, L.b1, 4 * d, w.hid, 1, 0));
+        WX_TRY(residual(w.hid, 4 * d, L.w2, L.w2_pk, L.b2, s_fc2, last ? e->declnf_g : e->dec[i + 1].ln1_g, last ? e->declnf_b : e->dec[i + 1].ln1_b));
     }
-    if (!p->want_logits) return WX_OK;
-    WX_TRY(launch_layernorm(w.x, e->declnf_g, e->declnf_b, w.xn, dtp, R, d, st));
     GemmArgs g = gemm_basic(e, w.xn, d, e->tok_emb, R, e->vocab_pad, d);
     g.Wpk = e->tok_emb_pk;
     g.ep.out = p->d_logits; g.ep.out_dtype = DT_F32; g.ep.ldo = e->vocab_pad;

