@@ -237,7 +237,7 @@ int wx_stream_destroy(void* stream);
 
 /* ---- paged key/value cache and drafted decoding -----------------------------------------------------------------------------
  * NO COUNTERPART IN THE REFERENCE (its decoder keeps one dense cache per call).  For decoding that checks several drafted tokens
- * of every sequence in one pass (wx_draft_step runs the engine's own decoder this way) and for programs that keep their own paged
+ * of every sequence in one pass (wx_draft_logits runs the engine's own decoder this way) and for programs that keep their own paged
  * cache.  A cache is a description of buffers that the CALLER owns; nothing is allocated, no call waits for the GPU, and every call
  * may be captured into a graph.  A cache belongs to one stream of work at a time: calls on one cache must not overlap, and neither
  * may replays of graphs captured from them.
@@ -298,7 +298,8 @@ int wx_cache_compact(const wx_cache* c, int32_t* d_n_live, void* stream);
  * h / (n_head / n_kv_head).  Strides in elements: heads' rows are contiguous and 16-byte aligned.  Softmax and sums in fp32; bf16
  * caches round the probabilities to bf16 for the product with the values.  What masked rows hold (NaN, infinities) has no effect.
  * split_tokens: the committed tokens are cut into pieces that workgroups take side by side; 0 = by the size of the batch; > 0 = pieces
- * of that many tokens (rounded up to a multiple of 64), so that a sequence's result does not depend on what else is in the batch. */
+ * of that many tokens (rounded up to a tile of 16 to 64 tokens, and to a 256th of what a table holds), so that a sequence's result does
+ * not depend on what else is in the batch.  d_out may be d_q. */
 typedef struct {
     int32_t layer, n, n_nodes, n_head;
     const int32_t *d_seqs, *d_parents, *d_counts;
@@ -336,7 +337,9 @@ int wx_tree_verify(const wx_tree_check* a, void* stream);
  * row (i, j) of d_logits [n][n_nodes][wx_logit_stride()] receives what the model answers to node j (want_logits 0: nothing, the pass
  * only fills the cache, as for a prompt).  Slots have to be reserved n_nodes tokens ahead.  The lengths stay: wx_tree_verify and
  * wx_cache_commit follow (WhisperEngine.decode_draft is the whole loop).  The cache has the engine's precision and device, n_text_layer
- * layers, n_text_head heads of 64, and at most 512 tokens a slot, so that a sequence's numbers do not depend on what else is in the pass.
+ * layers, n_text_head heads of 64, and at most 512 tokens a slot.  In bf16 the number of rows chooses the matrix products, and with them the
+ * order of their sums.  bf16 engines that attend the encoder output (wx_cross_attention_form) project their windows' keys and values, and on
+ * first use allocate room for them, within the call: there it cannot be captured.
  * Positions past n_text_ctx - 1 are not embedded: keep the depth within them.  Serves upstream's greedy DecodingTask.run (inside
  * ref:speech_recognition.py:55), several tokens a pass. */
 typedef struct {

@@ -181,6 +181,59 @@ def test_every_size_of_pass(group, N, windows):
     assert dist(*seen["bf16"]) <= 0.5 * dist(seen["bf16"][1], seen["fp32"][1])
 
 
+@pytest.mark.parametrize("precision", ["fp32", "bf16"])
+def test_a_captured_pass(precision):
+    """a drafted step (reserve, pass, verification, commit) captured once and replayed, other ids each time, the same as eager steps"""
+    from whisper_amd.draft import verify_tree
+    eng, _, _ = make(precision, 2, windows=2)
+    try:
+        n, N = 2, 5
+        i32 = lambda a: torch.tensor(np.ascontiguousarray(a), dtype=torch.int32, device="cuda")  # noqa: E731
+        par, slots, tok = i32([[-1, 0, 0, 1, 3]] * n), i32([1, 0]), i32(np.zeros((n, N)))
+        caches = [eng.draft_cache(n) for _ in range(2)]
+
+        def step(cache):
+            cache.reserve(slots, N)
+            logits = eng.draft_logits(cache, slots, tok, par)
+            r = verify_tree(logits, tok, par)
+            cache.commit(slots, r["path"], r["n_accept"])
+            return logits, r
+        ids = [np.random.RandomState(i).randint(0, 300, (n, N)) for i in range(5)]
+        tok.copy_(i32(ids[0]))
+        for c in caches:                                             # warm
+            step(c)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits, r = step(caches[0])
+        for x in ids[1:]:
+            tok.copy_(i32(x))
+            want = step(caches[1])
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(logits, want[0]) and all(torch.equal(r[k], want[1][k]) for k in r)
+            assert torch.equal(caches[0].lens, caches[1].lens)
+    finally:
+        eng.close()
+
+
+def test_no_capture_where_keys_are_projected():
+    from whisper_amd._lib import WxError
+    eng, _, _ = make("bf16", 32, windows=1)
+    try:
+        assert eng.cross_form == "encoder_output"
+        cache, one = eng.draft_cache(1), torch.zeros(1, dtype=torch.int32, device="cuda")
+        cache.reserve(one, 1)
+        eng.draft_logits(cache, one, one.view(1, 1))
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            one.add_(0)
+            with pytest.raises(WxError, match="captured"):
+                eng.draft_logits(cache, one, one.view(1, 1))
+    finally:
+        eng.close()
+
+
 def test_windows_path_with_ngram_drafts():
     eng, mel, _ = make(max_batch=2, windows=3)
     try:

@@ -238,6 +238,26 @@ def test_other_stream_and_replayed_graph():
         assert torch.equal(out, eager)
 
 
+def test_a_fixed_cut_does_not_see_the_batch():
+    """32-bit results of long sequences in pieces of a fixed length, alone and among many: the pieces are merged in the same order"""
+    lens = np.random.RandomState(3).randint(0, 3000, 40)
+    lens[5], lens[7] = 3000, 2999
+    c = Case(lens, 16, 8, 2, 64, 16, torch.float32, seed=8)
+    both = c.run(split_tokens=64)
+    c.check(both)
+    c.append = False
+    for i in (5, 7, 39):
+        one = c.cache.attend(c.layer, i32(c.slots[i:i + 1]), c.q[i:i + 1].cuda(), parents=i32(c.par[i:i + 1]), split_tokens=64)
+        assert torch.equal(one[0], both[i])
+
+
+def test_the_output_may_be_the_queries():
+    c = Case([700, 3, 90, 0], 9, 6, 2, 64, 16, BF16, seed=9)
+    q = c.q.cuda()
+    assert c.run(q=q, out=q) is q
+    c.check(q)
+
+
 def test_offsets_past_32_bits():
     """the last layer and the last pages of pools of 9 GB: the same results as in a small pool, and pages copied, appended to and moved there"""
     H, D, PS, L, P = 8, 128, 64, 3, 24000

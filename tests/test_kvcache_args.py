@@ -29,7 +29,7 @@ def check(**kw):
     return _lib.WxTreeCheck(**base)
 
 
-@pytest.mark.parametrize("kw", [dict(d_k=0), dict(d_table=0), dict(d_work=0), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(head_dim=80),
+@pytest.mark.parametrize("kw", [dict(d_k=0), dict(d_table=0), dict(d_work=0), dict(page_size=8), dict(n_pages=0x40000000), dict(page_size=48), dict(page_size=512), dict(head_dim=80),
                                 dict(n_pages=0), dict(max_seqs=0), dict(max_seqs=8193), dict(max_pages=0), dict(precision=2), dict(n_layer=0),
                                 dict(n_kv_head=0), dict(d_k=A + 4), dict(d_refs=A + 8), dict(max_pages=1 << 28)])
 def test_bad_cache_is_refused_by_every_call(kw):

@@ -1520,6 +1520,11 @@ int wx_draft_logits(wx_engine* e, const wx_cache* c, const wx_draft_pass* p, voi
     hipStream_t st = (hipStream_t)stream;
     const int d = e->d, dtp = e->dt, T = e->T, R = (int)rows64, windows = p->n / p->group, per_window = p->group * p->n_nodes;
     const size_t es = dtype_size(dtp);
+    if (e->xattn) {                                       // a replay would not project the keys and values of the windows encoded by then
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        HIP_TRY(hipStreamIsCapturing(st, &cs));
+        if (cs != hipStreamCaptureStatusNone) return fail(WX_ERR_STATE, "a drafted pass cannot be captured on an engine that attends the encoder output");
+    }
     if (!e->crossK || (e->xattn && e->cross_kv_B < windows)) { if (int r = project_cross_kv(e, e->encoded_B, st)) return r; }
     const DraftWork w = draft_work(e, R, (char*)p->d_work);
     const size_t cross_layer = (size_t)k.max_batch * e->Ht * T * HEAD_DIM;

@@ -48,7 +48,7 @@ const char* cache_fault(const wx_cache* c) {
         return "page_size must be 16, 32, 64, 128 or 256";
     if (c->head_dim != 64 && c->head_dim != 128) return "head_dim must be 64 or 128";
     if (c->precision != WX_PREC_F32 && c->precision != WX_PREC_BF16) return "bad precision";
-    if (c->n_kv_head > 4096 || c->n_layer > 4096 || (int64_t)c->max_pages * c->page_size > 0x3fffffff || (int64_t)c->max_seqs * c->max_pages > 0x7fffffff)
+    if (c->n_kv_head > 4096 || c->n_layer > 4096 || c->n_pages > 0x3fffffff || (int64_t)c->max_pages * c->page_size > 0x3fffffff || (int64_t)c->max_seqs * c->max_pages > 0x7fffffff)
         return "cache dimensions too large";
     if (((uintptr_t)c->d_k | (uintptr_t)c->d_v | (uintptr_t)c->d_refs | (uintptr_t)c->d_work) & 15) return "cache buffers must be 16-byte aligned";
     return nullptr;

@@ -1122,9 +1122,11 @@ static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeFo
     p.slots = p.single ? a.n : p.per ? (int)(a.n * ((most + p.per - 1) / p.per)) : p.takers;
     p.pieces = p.single ? 0 : p.per ? p.slots : p.takers + a.n;
     // the merge: as few rows a workgroup (as many threads on a row's pieces) as leave it at most 2048 workgroups (6 sequences of up to 38255
-    // tokens, 2 heads of 64, f32, shares of 128: 55 us so, 67 with every row's pieces on one group of threads)
+    // tokens, 2 heads of 64, f32, shares of 128: 55 us so, 67 with every row's pieces on one group of threads); the order of the sum follows from
+    // it, so with `per` it is taken for 8 sequences whatever their number
+    const int64_t merges = units * (p.per ? 8 : a.n);
     p.merge_rows = 1024 / c.head_dim;
-    while (p.merge_rows > 1 && units * a.n * ((rows + p.merge_rows / 2 - 1) / (p.merge_rows / 2)) <= 2048 * (int64_t)p.row_blocks) p.merge_rows /= 2;
+    while (p.merge_rows > 1 && merges * ((rows + p.merge_rows / 2 - 1) / (p.merge_rows / 2)) <= 2048 * (int64_t)p.row_blocks) p.merge_rows /= 2;
     return p;
 }
 static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {

@@ -19,6 +19,7 @@ The reference keeps one dense cache per call inside the model (ref:app/transcrip
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional, Union
 
 import torch
@@ -91,6 +92,13 @@ class PagedKVCache:
             raise ValueError(f"{what} must be a contiguous int32 tensor {want} on {self.device}")
         return t
 
+    @staticmethod
+    def _int(x, what: str, least: int = 0, below: int = 1 << 31) -> int:
+        x = operator.index(x)                                       # ctypes would cut a number to 32 bits without a word
+        if not least <= x < below:
+            raise ValueError(f"{what} must be {least} .. {below - 1}")
+        return x
+
     def _rows(self, t: torch.Tensor, what: str, shape: tuple) -> torch.Tensor:
         if t.dtype != self.dtype or t.device != self.device or tuple(t.shape) != shape:
             raise ValueError(f"{what} must be {self.dtype} {list(shape)} on {self.device}")
@@ -130,7 +138,11 @@ class PagedKVCache:
         are taken lowest number first, in the order of the list; status -3 where they run out."""
         seqs = self._ids(seqs, "seqs")
         n = seqs.shape[0]
-        each = None if isinstance(extra, int) else self._ids(extra, "extra", n)
+        each = None
+        if hasattr(extra, "__index__") and not torch.is_tensor(extra):
+            extra = self._int(extra, "extra")
+        else:
+            each = self._ids(extra, "extra", n)
         status = torch.empty_like(seqs)
         _check(self.lib.wx_cache_reserve(self._ref, seqs.data_ptr(), None if each is None else each.data_ptr(), extra if each is None else 0, n,
                                          status.data_ptr(), _raw_stream(self._index)), "wx_cache_reserve")
@@ -143,6 +155,8 @@ class PagedKVCache:
         n = seqs.shape[0]
         if k.dim() != (5 if layer is None else 4):
             raise ValueError("k and v must be [n_layers, n, n_nodes, n_kv_heads, head_dim], or without n_layers for one layer")
+        if layer is not None:
+            layer = self._int(layer, "layer", 0, self.n_layers)
         lead = (self.n_layers,) if layer is None else ()
         shape = (*lead, n, k.shape[-3], self.n_kv_heads, self.head_dim)
         k, v = self._rows(k, "k", shape), self._rows(v, "v", shape)
@@ -186,6 +200,7 @@ class PagedKVCache:
         if q.dim() != 4:
             raise ValueError("q must be [n, n_nodes, n_heads, head_dim]")
         nodes, heads = q.shape[1], q.shape[2]
+        layer, split_tokens = self._int(layer, "layer", 0, self.n_layers), self._int(split_tokens, "split_tokens")
         q = self._rows(q, "q", (n, nodes, heads, self.head_dim))
         if (k is None) != (v is None):
             raise ValueError("k and v come together")

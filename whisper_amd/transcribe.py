@@ -154,7 +154,7 @@ def transcribe(audio, language: Optional[str] = None, prompt: Union[None, str, S
     cmode = (_STATE["settings"] or {}).get("confidence_mode", "reference")
     lang_idx = None if language is None else language_index(language, eng.dims.n_vocab)
     if mode == "sequential":
-        if "draft" in decode_kw:
+        if decode_kw.pop("draft", None) is not None:
             raise ValueError("draft needs mode='windows' (the sequential loop decodes with timestamps)")
         from .longform import transcribe_sequential
         r = transcribe_sequential(eng, [pcm_host], tokenizer.decode, language_index=lang_idx,
