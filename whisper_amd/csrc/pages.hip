@@ -12,17 +12,20 @@ namespace wx {
 constexpr int PG_MAX_SEQS = 8192;
 constexpr int PG_NT = 1024;            // workgroup of the bookkeeping scans
 
+// (small: a launch costs the host 2.6 us with 8 bytes of arguments, 3.3 with 320)
 struct PageArgs {
     wx_cache c;
-    const int32_t *seqs, *src, *lens, *extra, *path, *counts;
-    int32_t* status;
+    const int32_t *seqs, *list, *path;   // list: sources (fork), lengths (truncate), tokens (reserve), counts (append, commit)
+    int32_t* out;                        // status of every entry; compaction: number of live pages
     int n, n_extra, n_nodes;
-    // append
+    int per_group;                       // layers a workgroup
+    int es;                              // bytes an element
+};
+struct AppendArgs {
+    PageArgs a;
     const char *rk, *rv;
     int64_t ks[4], vs[4];
-    int layer0, n_layers, per_group;   // per_group: layers a workgroup
-    int es;                            // bytes an element
-    int32_t* n_live;
+    int layer0, n_layers;
 };
 
 // ---- work buffer: one part for each purpose (include/whisper_amd.h: never kept between calls) ---------------------------------
@@ -72,9 +75,9 @@ __global__ __launch_bounds__(128) void cache_truncate_kernel(PageArgs a) {
     bool ok = entry_ok(a.seqs, i, c.max_seqs);
     const int s = a.seqs[i];
     int len = 0, held = 0, want = 0;
-    if (ok) { len = c.d_lens[s]; held = min(c.d_held[s], c.max_pages); want = a.lens ? a.lens[i] : 0; ok = want >= 0 && want <= len; }
+    if (ok) { len = c.d_lens[s]; held = min(c.d_held[s], c.max_pages); want = a.list ? a.list[i] : 0; ok = want >= 0 && want <= len; }
     __syncthreads();
-    if (threadIdx.x == 0 && a.status) a.status[i] = ok ? WX_OK : WX_ERR_INVALID;
+    if (threadIdx.x == 0 && a.out) a.out[i] = ok ? WX_OK : WX_ERR_INVALID;
     if (!ok) return;
     const int keep = (want + c.page_size - 1) / c.page_size;
     int32_t* row = c.d_table + (int64_t)s * c.max_pages;
@@ -85,7 +88,7 @@ __global__ __launch_bounds__(128) void cache_truncate_kernel(PageArgs a) {
 // ---- fork: all sources are read (and their pages counted up) before any destination is written -----------------------------------
 __global__ __launch_bounds__(128) void cache_fork_read_kernel(PageArgs a) {
     const wx_cache& c = a.c;
-    const int i = blockIdx.x, src = a.src[i];
+    const int i = blockIdx.x, src = a.list[i];
     const bool ok = entry_ok(a.seqs, i, c.max_seqs) && src >= 0 && src < c.max_seqs;
     int32_t* to = w_rows(c) + (int64_t)i * (c.max_pages + 2);
     if (!ok) { if (threadIdx.x == 0) to[0] = -1; return; }
@@ -103,7 +106,7 @@ __global__ __launch_bounds__(128) void cache_fork_write_kernel(PageArgs a) {
     const int i = blockIdx.x;
     const int32_t* from = w_rows(c) + (int64_t)i * (c.max_pages + 2);
     const int len = from[0];
-    if (threadIdx.x == 0 && a.status) a.status[i] = len < 0 ? WX_ERR_INVALID : WX_OK;
+    if (threadIdx.x == 0 && a.out) a.out[i] = len < 0 ? WX_ERR_INVALID : WX_OK;
     if (len < 0) return;
     const int s = a.seqs[i], keep = from[1], held = min(c.d_held[s], c.max_pages);
     __syncthreads();
@@ -124,21 +127,21 @@ __global__ __launch_bounds__(1024) void cache_fork_small_kernel(PageArgs a) {
     const wx_cache& c = a.c;
     const int tid = threadIdx.x, MP = c.max_pages, n = a.n;
     for (int i = tid; i < n; i += 1024) {
-        const int d = a.seqs[i], src = a.src[i];
+        const int d = a.seqs[i], src = a.list[i];
         bool ok = d >= 0 && d < c.max_seqs && src >= 0 && src < c.max_seqs;
         for (int j = 0; j < i; ++j) ok &= a.seqs[j] != d;
         const int len = ok ? c.d_lens[src] : -1;
         s_len[i] = len;
         s_keep[i] = len < 0 ? 0 : min((len + c.page_size - 1) / c.page_size, min(c.d_held[src], MP));
         s_held[i] = len < 0 ? 0 : min(c.d_held[d], MP);
-        if (a.status) a.status[i] = len < 0 ? WX_ERR_INVALID : WX_OK;
+        if (a.out) a.out[i] = len < 0 ? WX_ERR_INVALID : WX_OK;
     }
     __syncthreads();
     for (int u = tid; u < n * MP; u += 1024) {
         const int i = u / MP, q = u % MP;
         int page = -1;
         if (q < s_keep[i]) {
-            page = c.d_table[(int64_t)a.src[i] * MP + q];
+            page = c.d_table[(int64_t)a.list[i] * MP + q];
             if ((unsigned)page < (unsigned)c.n_pages) atomicAdd(&c.d_refs[page], 1);
         }
         cells[u] = page;
@@ -187,7 +190,7 @@ __global__ __launch_bounds__(PG_NT) void cache_reserve_kernel(PageArgs a) {
         const int i = i0 + tid;
         int need = 0, copy = 0, st = WX_ERR_INVALID;
         if (i < a.n) {
-            const int s = a.seqs[i], extra = a.extra ? a.extra[i] : a.n_extra;
+            const int s = a.seqs[i], extra = a.list ? a.list[i] : a.n_extra;
             if (s >= 0 && s < c.max_seqs && owner[s] == i && extra >= 0) {
                 const int len = c.d_lens[s], held = c.d_held[s];
                 const int64_t want = ((int64_t)len + extra + PS - 1) / PS;
@@ -229,7 +232,7 @@ __global__ __launch_bounds__(PG_NT) void cache_reserve_kernel(PageArgs a) {
         if (st == WX_OK && need > 0 && first + need > found) st = WX_ERR_NOMEM;
         const bool go = st == WX_OK && need > 0;
         if (lane == 0) {
-            if (a.status) a.status[i] = st;
+            if (a.out) a.out[i] = st;
             pairs[4 * i] = -1;
         }
         if (!go) continue;
@@ -286,11 +289,12 @@ __device__ __forceinline__ bool rows_private(const wx_cache& c, int s, int len, 
 // values through the layers, two layers' loads at a time.  Bound by the copy: 64 x 16 rows (769 there), 32 layers x 20 heads of 64: 252 MB in
 // 55 us, 4.6 TB/s.
 constexpr int AP_NODES = 4;
-__global__ __launch_bounds__(256) void cache_append_kernel(PageArgs a) {
+__global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs b) {
     __shared__ int64_t place[AP_NODES];
+    const PageArgs& a = b.a;
     const wx_cache& c = a.c;
     const int i = blockIdx.x, j0 = blockIdx.y * AP_NODES;
-    const int count = a.counts ? min(a.counts[i], a.n_nodes) : a.n_nodes;
+    const int count = a.list ? min(a.list[i], a.n_nodes) : a.n_nodes;
     if (j0 >= count || !entry_ok(a.seqs, i, c.max_seqs)) return;
     const int s = a.seqs[i], len = c.d_lens[s];
     if (!rows_private(c, s, len, count)) return;
@@ -301,14 +305,14 @@ __global__ __launch_bounds__(256) void cache_append_kernel(PageArgs a) {
         place[threadIdx.x] = c.d_table[(int64_t)s * c.max_pages + t / c.page_size] * page_b + (t % c.page_size) * row_b;
     }
     __syncthreads();
-    const int l0 = blockIdx.z * a.per_group, l1 = min(a.n_layers, l0 + a.per_group);
+    const int l0 = blockIdx.z * a.per_group, l1 = min(b.n_layers, l0 + a.per_group);
     for (int u = threadIdx.x; u < nodes * heads * per; u += 256) {
         const int x = u % per, h = (u / per) % heads, j = u / (per * heads);
-        const char* k = a.rk + (l0 * a.ks[0] + i * a.ks[1] + (j0 + j) * a.ks[2] + h * a.ks[3]) * a.es + x * 16;
-        const char* v = a.rv + (l0 * a.vs[0] + i * a.vs[1] + (j0 + j) * a.vs[2] + h * a.vs[3]) * a.es + x * 16;
-        const int64_t to = (a.layer0 + l0) * layer_b + place[j] + h * head_b + x * 16;
+        const char* k = b.rk + (l0 * b.ks[0] + i * b.ks[1] + (j0 + j) * b.ks[2] + h * b.ks[3]) * a.es + x * 16;
+        const char* v = b.rv + (l0 * b.vs[0] + i * b.vs[1] + (j0 + j) * b.vs[2] + h * b.vs[3]) * a.es + x * 16;
+        const int64_t to = (b.layer0 + l0) * layer_b + place[j] + h * head_b + x * 16;
         char *kt = (char*)c.d_k + to, *vt = (char*)c.d_v + to;
-        const int64_t kstep = a.ks[0] * a.es, vstep = a.vs[0] * a.es;
+        const int64_t kstep = b.ks[0] * a.es, vstep = b.vs[0] * a.es;
         int l = l0;
         for (; l + 1 < l1; l += 2, k += 2 * kstep, v += 2 * vstep, kt += 2 * layer_b, vt += 2 * layer_b) {
             const i32x4 k0 = *reinterpret_cast<const i32x4*>(k), k1 = *reinterpret_cast<const i32x4*>(k + kstep);
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(256) void cache_append_kernel(PageArgs a) {
 __device__ __forceinline__ bool commit_ok(const PageArgs& a, int i, int* taken) {
     const wx_cache& c = a.c;
     if (!entry_ok(a.seqs, i, c.max_seqs)) return false;
-    const int k = a.counts[i];
+    const int k = a.list[i];
     *taken = k;
     if (k < 0 || k > a.n_nodes) return false;
     const int32_t* path = a.path + (int64_t)i * a.n_nodes;
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(256) void cache_commit_rows_kernel(PageArgs a) {
     int taken;
     const bool ok = commit_ok(a, i, &taken);
     const bool all = gridDim.y == 1;
-    if (all && threadIdx.x == 0 && a.status) a.status[i] = ok ? WX_OK : WX_ERR_INVALID;
+    if (all && threadIdx.x == 0 && a.out) a.out[i] = ok ? WX_OK : WX_ERR_INVALID;
     if (!ok) return;
     const int s = a.seqs[i], len = c.d_lens[s];
     const int32_t* path = a.path + (int64_t)i * a.n_nodes;
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(64) void cache_commit_len_kernel(PageArgs a) {
     const bool ok = commit_ok(a, i, &taken);
     __syncthreads();
     if (threadIdx.x == 0) {
-        if (a.status) a.status[i] = ok ? WX_OK : WX_ERR_INVALID;
+        if (a.out) a.out[i] = ok ? WX_OK : WX_ERR_INVALID;
         if (ok) a.c.d_lens[a.seqs[i]] += taken;
     }
 }
@@ -430,7 +434,7 @@ __global__ __launch_bounds__(PG_NT) void cache_compact_plan_kernel(PageArgs a) {
         c.d_refs[hole[i]] = c.d_refs[from[i]];
         c.d_refs[from[i]] = 0;
     }
-    if (tid == 0) { *w_count(c) = moves; if (a.n_live) *a.n_live = live; }
+    if (tid == 0) { *w_count(c) = moves; if (a.out) *a.out = live; }
 }
 // grid (any number, layer, keys / values): whole pages
 __global__ __launch_bounds__(256) void cache_compact_move_kernel(PageArgs a) {
@@ -455,7 +459,7 @@ __global__ __launch_bounds__(256) void cache_compact_table_kernel(PageArgs a) {
 
 static PageArgs page_args(const wx_cache* c, const int32_t* seqs, int n, int32_t* status) {
     PageArgs a{};
-    a.c = *c; a.seqs = seqs; a.n = n; a.status = status;
+    a.c = *c; a.seqs = seqs; a.n = n; a.out = status;
     a.es = c->precision == WX_PREC_F32 ? 4 : 2;
     return a;
 }
@@ -480,7 +484,7 @@ int wx_cache_truncate(const wx_cache* c, const int32_t* d_seqs, const int32_t* d
     if (n == 0) return WX_OK;
     OnDevice on(c->device);
     PageArgs a = page_args(c, d_seqs, n, d_status);
-    a.lens = d_lens;
+    a.list = d_lens;
     hipLaunchKernelGGL(cache_truncate_kernel, dim3(n), dim3(128), 0, (hipStream_t)stream, a);
     PG_DONE();
 }
@@ -491,7 +495,7 @@ int wx_cache_fork(const wx_cache* c, const int32_t* d_dst, const int32_t* d_src,
     if (!d_src) return set_error(WX_ERR_INVALID, "null list of sources");
     OnDevice on(c->device);
     PageArgs a = page_args(c, d_dst, n, d_status);
-    a.src = d_src;
+    a.list = d_src;
     if (n <= FK_ENTRIES && (int64_t)n * c->max_pages <= FK_CELLS) {
         hipLaunchKernelGGL(cache_fork_small_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
         PG_DONE();
@@ -507,7 +511,7 @@ int wx_cache_reserve(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_
     if (n == 0) return WX_OK;
     OnDevice on(c->device);
     PageArgs a = page_args(c, d_seqs, n, d_status);
-    a.extra = d_extra; a.n_extra = extra;
+    a.list = d_extra; a.n_extra = extra;
     hipLaunchKernelGGL(cache_reserve_kernel, dim3(1), dim3(PG_NT), 0, (hipStream_t)stream, a);
     hipLaunchKernelGGL(cache_copy_tail_kernel, dim3(n, c->n_layer, 2), dim3(256), 0, (hipStream_t)stream, a);
     PG_DONE();
@@ -520,20 +524,22 @@ int wx_cache_append(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_c
     if (n_nodes < 0 || n_nodes > 65536) return set_error(WX_ERR_INVALID, "n_nodes must be 0 .. 65536");
     if (n == 0 || n_nodes == 0) return WX_OK;
     if (!d_k || !d_v || !k_strides || !v_strides) return set_error(WX_ERR_INVALID, "null rows");
-    PageArgs a = page_args(c, d_seqs, n, nullptr);
+    AppendArgs b{};
+    PageArgs& a = b.a;
+    a = page_args(c, d_seqs, n, nullptr);
     const int unit = 16 / a.es;
     for (int i = 0; i < 4; ++i) {
-        a.ks[i] = k_strides[i]; a.vs[i] = v_strides[i];
-        if (a.ks[i] < 0 || a.vs[i] < 0 || a.ks[i] % unit || a.vs[i] % unit) return set_error(WX_ERR_INVALID, "row strides must be >= 0 and multiples of 16 bytes");
+        b.ks[i] = k_strides[i]; b.vs[i] = v_strides[i];
+        if (b.ks[i] < 0 || b.vs[i] < 0 || b.ks[i] % unit || b.vs[i] % unit) return set_error(WX_ERR_INVALID, "row strides must be >= 0 and multiples of 16 bytes");
     }
     if (((uintptr_t)d_k | (uintptr_t)d_v) & 15) return set_error(WX_ERR_INVALID, "rows must be 16-byte aligned");
     OnDevice on(c->device);
-    a.counts = d_counts; a.n_nodes = n_nodes; a.layer0 = layer0; a.n_layers = n_layers; a.rk = (const char*)d_k; a.rv = (const char*)d_v;
+    a.list = d_counts; a.n_nodes = n_nodes; b.layer0 = layer0; b.n_layers = n_layers; b.rk = (const char*)d_k; b.rv = (const char*)d_v;
     // as many layers a workgroup as leave 2048 workgroups (8 on every CU): the look-up is paid once for them
     const int groups = (n_nodes + AP_NODES - 1) / AP_NODES;
     const int64_t z = (2048 + (int64_t)n * groups - 1) / ((int64_t)n * groups);
     a.per_group = (int)((n_layers + z - 1) / z);
-    hipLaunchKernelGGL(cache_append_kernel, dim3(n, groups, (n_layers + a.per_group - 1) / a.per_group), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(cache_append_kernel, dim3(n, groups, (n_layers + a.per_group - 1) / a.per_group), dim3(256), 0, (hipStream_t)stream, b);
     PG_DONE();
 }
 
@@ -545,7 +551,7 @@ int wx_cache_commit(const wx_cache* c, const int32_t* d_seqs, const int32_t* d_p
     if (!d_counts || (n_nodes > 0 && !d_path)) return set_error(WX_ERR_INVALID, "null path or counts");
     OnDevice on(c->device);
     PageArgs a = page_args(c, d_seqs, n, d_status);
-    a.path = d_path; a.counts = d_counts; a.n_nodes = n_nodes;
+    a.path = d_path; a.list = d_counts; a.n_nodes = n_nodes;
     // one workgroup an entry where a token's rows of all layers are at most 32 KiB: no second launch for the lengths
     const int64_t token_b = 2 * (int64_t)c->n_layer * c->n_kv_head * c->head_dim * a.es;
     const int64_t y = token_b <= 32768 ? 1 : (1024 + n - 1) / n;
@@ -560,7 +566,7 @@ int wx_cache_compact(const wx_cache* c, int32_t* d_n_live, void* stream) {
     PG_CHECK(c);
     OnDevice on(c->device);
     PageArgs a = page_args(c, nullptr, 0, nullptr);
-    a.n_live = d_n_live;
+    a.out = d_n_live;
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(cache_compact_plan_kernel, dim3(1), dim3(PG_NT), 0, st, a);
     const int64_t cells = (int64_t)c->max_seqs * c->max_pages;

@@ -86,7 +86,7 @@ class PagedKVCache:
         if not torch.is_tensor(t):
             t = torch.tensor(list(t), dtype=torch.int32, device=self.device)
         shape = t.shape
-        if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous() or len(shape) != (1 if cols is None else 2) or \
+        if t.dtype is not torch.int32 or t.get_device() != self._index or not t.is_contiguous() or len(shape) != (1 if cols is None else 2) or \
                 (n is not None and shape[0] != n) or (cols is not None and shape[1] != cols):
             want = f"[{'n' if n is None else n}{'' if cols is None else f', {cols}'}]"
             raise ValueError(f"{what} must be a contiguous int32 tensor {want} on {self.device}")
