@@ -251,6 +251,25 @@ def test_a_fixed_cut_does_not_see_the_batch():
         assert torch.equal(one[0], both[i])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("L", [2000, 16384])
+def test_one_long_piece_in_32_bits(D, L):
+    """one workgroup takes the whole sequence: the root mean square of the error, against that of the result.  A wave adds up a quarter of the
+    keys; every addition is off by half a step, 2^-24, of a sum that grows as a random walk does: 2^-24 sqrt(L / 4 / 2) of the result.  Scores
+    and exponentials add a few steps that do not grow with L."""
+    H, pages = 2, L // 16 + 1
+    g = torch.Generator().manual_seed(L + D)
+    c = PagedKVCache.allocate(1, H, D, pages, 1, pages, dtype=torch.float32)
+    k, v = (torch.randn(pages, H, 16, D, generator=g) for _ in range(2))
+    c.k[0], c.v[0] = k.cuda(), v.cuda()
+    c.table.copy_(i32([range(pages)])); c.refs.fill_(1); c.held.fill_(pages); c.lens.fill_(L - 1)
+    q = torch.randn(1, 1, 3 * H, D, generator=g)
+    got = c.attend(0, i32([0]), q.cuda(), split_tokens=1 << 20)[0, 0].cpu().double()
+    K, V = (x.permute(1, 0, 2, 3).reshape(H, -1, D)[:, :L].double() for x in (k, v))
+    want = (torch.softmax(q[0, 0].view(H, 3, D).double() @ K.transpose(1, 2) * D ** -0.5, -1) @ V).reshape(3 * H, D)
+    assert float(((got - want) ** 2).sum().sqrt() / (want ** 2).sum().sqrt()) <= 2.0 ** -24 * ((L / 8) ** 0.5 + 16)
+
+
 def test_the_output_may_be_the_queries():
     c = Case([700, 3, 90, 0], 9, 6, 2, 64, 16, BF16, seed=9)
     q = c.q.cuda()

@@ -282,7 +282,9 @@ template <int D, int RT> struct RowState {
             mt = fmaxf(mt, __shfl_xor(mt, 16));
             mt = fmaxf(mt, __shfl_xor(mt, 32));
             const float mn = fmaxf(m[t], mt), base = mn == -INFINITY ? 0.f : mn * c;
-            const float alpha = __builtin_amdgcn_exp2f(fmaf(m[t], c, -base));       // m = -infinity: 0
+            // 1 while the maximum stands: m c - base is the rounding of base, and its power, tile after tile, would weigh early keys by another
+            // factor than late ones (16384 tokens in one piece, f32: 1.1e-5 off, 1.2e-6 without)
+            const float alpha = mn == m[t] ? 1.f : __builtin_amdgcn_exp2f((m[t] - mn) * c);       // m = -infinity: 0
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < NS; ++k)
