@@ -269,21 +269,6 @@ __global__ __launch_bounds__(256) void cache_copy_tail_kernel(PageArgs a) {
     }
 }
 
-// rows [len, len + upto) of a slot: reserved, on pages of the pool that no other slot holds (every thread of the workgroup)
-__device__ __forceinline__ bool rows_private(const wx_cache& c, int s, int len, int upto) {
-    if (upto <= 0) return true;
-    const int64_t held = min(c.d_held[s], c.max_pages);
-    int bad = len < 0 || (int64_t)len + upto > held * c.page_size;
-    if (!bad) {
-        const int32_t* row = c.d_table + (int64_t)s * c.max_pages;
-        for (int p = len / c.page_size + threadIdx.x; p <= (len + upto - 1) / c.page_size; p += blockDim.x) {
-            const int page = row[p];
-            if ((unsigned)page >= (unsigned)c.n_pages || c.d_refs[page] != 1) bad = 1;
-        }
-    }
-    return !__syncthreads_or(bad);
-}
-
 // ---- append: grid (entry, group of AP_NODES nodes, group of layers) -------------------------------------------------------------------
 // The entry is checked and its places are looked up once for all layers of the group; a thread then takes its 16 bytes of keys and of
 // values through the layers, two layers' loads at a time.  Bound by the copy: 64 x 16 rows (769 there), 32 layers x 20 heads of 64: 252 MB in
@@ -293,56 +278,79 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs b) {
     __shared__ int64_t place[AP_NODES];
     const PageArgs& a = b.a;
     const wx_cache& c = a.c;
-    const int i = blockIdx.x, j0 = blockIdx.y * AP_NODES;
-    const int count = a.list ? min(a.list[i], a.n_nodes) : a.n_nodes;
-    if (j0 >= count || !entry_ok(a.seqs, i, c.max_seqs)) return;
-    const int s = a.seqs[i], len = c.d_lens[s];
-    if (!rows_private(c, s, len, count)) return;
-    const int64_t row_b = (int64_t)c.head_dim * a.es, head_b = row_b * c.page_size, page_b = head_b * c.n_kv_head, layer_b = page_b * c.n_pages;
-    const int nodes = min(AP_NODES, count - j0), per = (int)(row_b / 16), heads = c.n_kv_head;
-    if (threadIdx.x < nodes) {
-        const int t = len + j0 + threadIdx.x;
-        place[threadIdx.x] = c.d_table[(int64_t)s * c.max_pages + t / c.page_size] * page_b + (t % c.page_size) * row_b;
-    }
-    __syncthreads();
+    const int i = blockIdx.x, j0 = blockIdx.y * AP_NODES, tid = threadIdx.x;
     const int l0 = blockIdx.z * a.per_group, l1 = min(b.n_layers, l0 + a.per_group);
-    for (int u = threadIdx.x; u < nodes * heads * per; u += 256) {
-        const int x = u % per, h = (u / per) % heads, j = u / (per * heads);
-        const char* k = b.rk + (l0 * b.ks[0] + i * b.ks[1] + (j0 + j) * b.ks[2] + h * b.ks[3]) * a.es + x * 16;
-        const char* v = b.rv + (l0 * b.vs[0] + i * b.vs[1] + (j0 + j) * b.vs[2] + h * b.vs[3]) * a.es + x * 16;
-        const int64_t to = (b.layer0 + l0) * layer_b + place[j] + h * head_b + x * 16;
+    const int64_t row_b = (int64_t)c.head_dim * a.es, head_b = row_b * c.page_size, page_b = head_b * c.n_kv_head, layer_b = page_b * c.n_pages;
+    const int per = (int)(row_b / 16), heads = c.n_kv_head;
+    const int64_t kstep = b.ks[0] * a.es, vstep = b.vs[0] * a.es;
+    auto k_at = [&](int u) { const int x = u % per, h = (u / per) % heads, j = u / (per * heads); return b.rk + (l0 * b.ks[0] + i * b.ks[1] + (j0 + j) * b.ks[2] + h * b.ks[3]) * a.es + x * 16; };
+    auto v_at = [&](int u) { const int x = u % per, h = (u / per) % heads, j = u / (per * heads); return b.rv + (l0 * b.vs[0] + i * b.vs[1] + (j0 + j) * b.vs[2] + h * b.vs[3]) * a.es + x * 16; };
+    // the thread's first rows are on their way while the entry is looked up
+    i32x4 k0 = {0, 0, 0, 0}, v0 = k0, k1 = k0, v1 = k0;
+    auto load = [&](const char* k, const char* v, bool two) {
+        k0 = *reinterpret_cast<const i32x4*>(k); v0 = *reinterpret_cast<const i32x4*>(v);
+        if (two) { k1 = *reinterpret_cast<const i32x4*>(k + kstep); v1 = *reinterpret_cast<const i32x4*>(v + vstep); }
+    };
+    const int s = a.seqs[i], count = a.list ? min(a.list[i], a.n_nodes) : a.n_nodes, nodes = min(AP_NODES, count - j0);
+    if (tid < nodes * heads * per) load(k_at(tid), v_at(tid), l0 + 1 < l1);
+    int bad = 0;
+    for (int j = tid; j < i; j += 256) bad |= a.seqs[j] == s;
+    if (j0 >= count || s < 0 || s >= c.max_seqs) return;
+    const int len = c.d_lens[s], held = min(c.d_held[s], c.max_pages);
+    if (len < 0 || (int64_t)len + count > (int64_t)held * c.page_size) return;
+    const int32_t* row = c.d_table + (int64_t)s * c.max_pages;
+    if (tid < nodes) {
+        const int t = len + j0 + tid;
+        place[tid] = row[t / c.page_size] * page_b + (t % c.page_size) * row_b;                  // (used if the pages are found right)
+    }
+    for (int q = len / c.page_size + tid; q <= (len + count - 1) / c.page_size; q += 256) {
+        const int page = row[q];
+        if ((unsigned)page >= (unsigned)c.n_pages || c.d_refs[page] != 1) bad = 1;
+    }
+    if (__syncthreads_or(bad)) return;
+    for (int u = tid; u < nodes * heads * per; u += 256) {
+        const char *k = k_at(u), *v = v_at(u);
+        const int64_t to = (b.layer0 + l0) * layer_b + place[u / (per * heads)] + (u / per) % heads * head_b + u % per * 16;
         char *kt = (char*)c.d_k + to, *vt = (char*)c.d_v + to;
-        const int64_t kstep = b.ks[0] * a.es, vstep = b.vs[0] * a.es;
-        int l = l0;
-        for (; l + 1 < l1; l += 2, k += 2 * kstep, v += 2 * vstep, kt += 2 * layer_b, vt += 2 * layer_b) {
-            const i32x4 k0 = *reinterpret_cast<const i32x4*>(k), k1 = *reinterpret_cast<const i32x4*>(k + kstep);
-            const i32x4 v0 = *reinterpret_cast<const i32x4*>(v), v1 = *reinterpret_cast<const i32x4*>(v + vstep);
-            *reinterpret_cast<i32x4*>(kt) = k0; *reinterpret_cast<i32x4*>(kt + layer_b) = k1;
-            *reinterpret_cast<i32x4*>(vt) = v0; *reinterpret_cast<i32x4*>(vt + layer_b) = v1;
-        }
-        if (l < l1) {
-            const i32x4 k0 = *reinterpret_cast<const i32x4*>(k), v0 = *reinterpret_cast<const i32x4*>(v);
+        if (u != tid) load(k, v, l0 + 1 < l1);
+        for (int l = l0; l < l1; l += 2) {
+            const bool two = l + 1 < l1;
             *reinterpret_cast<i32x4*>(kt) = k0; *reinterpret_cast<i32x4*>(vt) = v0;
+            if (two) { *reinterpret_cast<i32x4*>(kt + layer_b) = k1; *reinterpret_cast<i32x4*>(vt + layer_b) = v1; }
+            k += 2 * kstep; v += 2 * vstep; kt += 2 * layer_b; vt += 2 * layer_b;
+            if (l + 2 < l1) load(k, v, l + 3 < l1);
         }
     }
 }
 
 // ---- commit ------------------------------------------------------------------------------------------------------------------------
-// Whether entry i's path may be followed (every thread of the workgroup); *taken = its length.
-__device__ __forceinline__ bool commit_ok(const PageArgs& a, int i, int* taken) {
+// Whether entry i's path may be followed (every thread of the workgroup); *taken = its length, *stay = how many of its first blockDim.x rows
+// stay where they are.  What depends on no other load is asked for first: list, count and path; then lengths; pages; their users.
+__device__ __forceinline__ bool commit_ok(const PageArgs& a, int i, int* taken, int* stay) {
     const wx_cache& c = a.c;
-    if (!entry_ok(a.seqs, i, c.max_seqs)) return false;
-    const int k = a.list[i];
-    *taken = k;
-    if (k < 0 || k > a.n_nodes) return false;
+    const int tid = threadIdx.x, nt = blockDim.x;
     const int32_t* path = a.path + (int64_t)i * a.n_nodes;
+    const int s = a.seqs[i], k = a.list[i];
+    const int mine = tid < a.n_nodes ? path[tid] : 0, before = tid > 0 && tid < a.n_nodes ? path[tid - 1] : -1;
     int bad = 0;
-    for (int j = threadIdx.x; j < k; j += blockDim.x) bad |= path[j] < 0 || (j > 0 && path[j] <= path[j - 1]);
-    if (__syncthreads_or(bad)) return false;
-    if (k == 0) return true;
-    const int last = path[k - 1];
-    if (last >= 0x40000000) return false;
-    return rows_private(c, a.seqs[i], c.d_lens[a.seqs[i]], last + 1);
+    for (int j = tid; j < i; j += nt) bad |= a.seqs[j] == s;
+    *taken = k;
+    if (s < 0 || s >= c.max_seqs || k < 0 || k > a.n_nodes) return false;
+    const int len = c.d_lens[s], held = min(c.d_held[s], c.max_pages), last = k > 0 ? path[k - 1] : 0;
+    bad |= tid < k && (mine < 0 || mine <= before);
+    for (int j = tid + nt; j < k; j += nt) bad |= path[j] < 0 || path[j] <= path[j - 1];
+    if (k > 0) {
+        if (len < 0 || last < 0 || (int64_t)len + last + 1 > (int64_t)held * c.page_size) bad = 1;
+        else {
+            const int32_t* row = c.d_table + (int64_t)s * c.max_pages;
+            for (int q = len / c.page_size + tid; q <= (len + last) / c.page_size; q += nt) {
+                const int page = row[q];
+                if ((unsigned)page >= (unsigned)c.n_pages || c.d_refs[page] != 1) bad = 1;
+            }
+        }
+    }
+    *stay = __syncthreads_count(tid < k && mine == tid);             // a path ascends: the first ones
+    return !__syncthreads_or(bad);
 }
 // grid (entry, group of layers): a thread takes 16 bytes of a head's rows of one layer, keys or values, down the whole path.  path[k] >= k
 // and ascends, so a row that is overwritten was read before by the same thread (eight rows are read before they are written); rows that
@@ -353,8 +361,8 @@ __global__ __launch_bounds__(256) void cache_commit_rows_kernel(PageArgs a) {
     __shared__ int64_t from[CM_ROWS], to[CM_ROWS];
     const wx_cache& c = a.c;
     const int i = blockIdx.x;
-    int taken;
-    const bool ok = commit_ok(a, i, &taken);
+    int taken, k0;
+    const bool ok = commit_ok(a, i, &taken, &k0);
     const bool all = gridDim.y == 1;
     if (all && threadIdx.x == 0 && a.out) a.out[i] = ok ? WX_OK : WX_ERR_INVALID;
     if (!ok) return;
@@ -363,8 +371,7 @@ __global__ __launch_bounds__(256) void cache_commit_rows_kernel(PageArgs a) {
     const int32_t* row = c.d_table + (int64_t)s * c.max_pages;
     const int64_t row_b = (int64_t)c.head_dim * a.es, head_b = row_b * c.page_size, page_b = head_b * c.n_kv_head, layer_b = page_b * c.n_pages;
     const int per = (int)(row_b / 16), cols = c.n_kv_head * per, l0 = blockIdx.y * a.per_group, layers = min(c.n_layer, l0 + a.per_group) - l0;
-    int k0 = 0;
-    while (k0 < taken && path[k0] == k0) ++k0;                        // (uniform; the rows of a draft whose first branch was taken stay)
+    if (k0 == blockDim.x) while (k0 < taken && path[k0] == k0) ++k0;  // (uniform)
     for (; k0 < taken; k0 += CM_ROWS) {
         const int moves = min(CM_ROWS, taken - k0);
         __syncthreads();
@@ -393,8 +400,8 @@ __global__ __launch_bounds__(256) void cache_commit_rows_kernel(PageArgs a) {
 }
 __global__ __launch_bounds__(64) void cache_commit_len_kernel(PageArgs a) {
     const int i = blockIdx.x;
-    int taken;
-    const bool ok = commit_ok(a, i, &taken);
+    int taken, stay;
+    const bool ok = commit_ok(a, i, &taken, &stay);
     __syncthreads();
     if (threadIdx.x == 0) {
         if (a.out) a.out[i] = ok ? WX_OK : WX_ERR_INVALID;
