@@ -108,6 +108,33 @@ def test_in_place_reorder_with_repeats():
         same(cache, model)
 
 
+@pytest.mark.parametrize("L,H", [(3, 2), (5, 16)])
+def test_long_paths(L, H):
+    """paths of hundreds of rows: some stay all along, some part early, late or behind the first 256, some are not paths behind the first 256"""
+    N, n, PS = 700, 6, 64
+    cache, model = make(L=L, H=H, PS=PS, pages=n * 12 + 1, seqs=n, width=12, dtype=torch.bfloat16)
+    grow(cache, model, [3, 0, 17, 60, 1, 9])
+    ids = list(range(n))
+    assert status(cache.reserve(i32(ids), N)) == model.reserve(ids, N) == [OK] * n
+    rows = torch.randn(L, n, N, H, 64, device="cuda").bfloat16()
+    counts = [N, N, 690, N, N, 301]
+    cache.append(i32(ids), rows, rows.flip(2), counts=i32(counts))
+    model.append(ids, rows.float().cpu().numpy(), rows.flip(2).float().cpu().numpy(), counts, list(range(L)))
+    same(cache, model)
+    rng = np.random.RandomState(0)
+    path = np.full((n, N), -1, np.int32)
+    path[0] = np.arange(N)
+    for i, stay in ((1, 0), (2, 200), (3, 256), (4, 400)):
+        take = np.concatenate([np.arange(stay), np.sort(rng.choice(np.arange(stay, 690), 280, replace=False))])
+        path[i, :len(take)] = take
+    path[5, :300] = np.arange(300)
+    path[5, 290] = 289
+    taken = [N, 280, 480, 536, 680, 300]
+    want = model.commit(ids, path, taken)
+    assert status(cache.commit(i32(ids), i32(path), i32(taken))) == want == [OK] * 5 + [INVALID]
+    same(cache, model)
+
+
 def test_refused_entries_change_nothing():
     cache, model = make(pages=7)
     grow(cache, model, [17, 16])
