@@ -103,6 +103,52 @@ def test_against_64_bits(dtype, lens, N, heads, kv_heads, D, PS, append):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("n,N,heads,kv_heads,D,longest", [(130, 1, 8, 8, 64, 500), (129, 5, 24, 8, 64, 90), (66, 16, 16, 16, 128, 140), (1100, 1, 4, 1, 64, 33), (35, 2, 60, 30, 128, 508),
+                                                          (70, 3, 24, 12, 128, 60)])
+def test_many_short_sequences(dtype, n, N, heads, kv_heads, D, longest):
+    """more sequences x heads than waves fit at once, short enough for a wave each: ragged, some empty, some padding, some refused"""
+    rng = np.random.RandomState(n + N)
+    c = Case(rng.randint(0, longest + 1, n), N, heads, kv_heads, D, 16, dtype, seed=n, counts=rng.randint(0, N + 1, n))
+    c.check(c.run())
+    c.append = False
+    before = c.run()
+    c.check(before)
+    slots = c.slots.copy()
+    slots[[3, 20]] = -1, n + 5
+    c.cache.refs[c.cache.table[int(slots[7]), 0]] = 2                          # (a page that is shared does not matter to a call that appends nothing)
+    got = c.cache.attend(c.layer, i32(slots), c.q.cuda(), parents=i32(c.par), counts=i32(c.counts))
+    assert not got[3].any() and torch.isnan(got[20]).all()
+    rest = [i for i in range(n) if i not in (3, 20)]
+    assert torch.equal(got[rest], before[rest])
+    # appending: a slot named twice and one whose page is shared are NaN, and leave the cache as it was
+    slots[30] = slots[31]
+    held = int(c.lens[7]) // 16
+    c.cache.refs[c.cache.table[int(slots[7]), held]] = 2
+    was = c.cache.k.clone()
+    kn, vn = torch.randn_like(c.kn).cuda(), torch.randn_like(c.vn).cuda()
+    got = c.cache.attend(c.layer, i32(slots), c.q.cuda(), parents=i32(c.par), counts=i32(c.counts), k=kn, v=vn)
+    for i in (7, 31):
+        assert torch.isnan(got[i]).all() if c.counts[i] > 0 else True
+        own = c.cache.table[int(c.slots[i]), :-(-(int(c.lens[i]) + N) // 16)].long()
+        if i == 7:
+            assert torch.equal(c.cache.k[:, own].nan_to_num(9.0), was[:, own].nan_to_num(9.0))
+    i = next(x for x in range(40, n) if c.counts[x] > 0) if n > 40 else 34
+    if c.counts[i] > 0:
+        page, row = int(c.cache.table[int(slots[i]), int(c.lens[i]) // 16]), int(c.lens[i]) % 16
+        assert torch.equal(c.cache.k[c.layer, page, :, row], kn[i, 0])
+
+
+@pytest.mark.parametrize("dtype,D,longest", [(torch.float32, 64, 300), (torch.float32, 64, 440), (BF16, 128, 300), (BF16, 128, 470)])
+def test_very_many_sequences(dtype, D, longest):
+    lens = np.random.RandomState(longest).randint(0, 21, 2001)
+    lens[[0, 1000, 2000]] = longest
+    c = Case(lens, 2, 2, 1, D, 16, dtype, seed=longest)
+    c.check(c.run())
+    c.append = False
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
 @pytest.mark.parametrize("n,N,heads,kv_heads,D,longest", [(1, 3, 1, 1, 64, 5000), (3, 2, 2, 1, 128, 3000), (8, 64, 8, 4, 64, 700), (17, 64, 8, 4, 64, 640), (33, 64, 8, 8, 64, 560),
                                                           (9, 33, 8, 4, 128, 700), (24, 33, 16, 8, 128, 530)])
 def test_many_pieces_and_many_rows(dtype, n, N, heads, kv_heads, D, longest):

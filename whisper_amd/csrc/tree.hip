@@ -165,31 +165,31 @@ __device__ __forceinline__ void tree_uniform(TreeJob& t) {
     UNI(ok); UNI(i); UNI(kh); UNI(rb); UNI(piece); UNI(whole); UNI(seq); UNI(len); UNI(count); UNI(n_pre); UNI(t0); UNI(t1); UNI(last);
 #undef UNI
 }
-// The one job of a workgroup that does one whole sequence: no search, and nothing waits for another wave.
+// The one job of a workgroup that does one whole sequence, or (solo >= 0) of its wave `solo`: no search, and nothing waits for another wave.
 template <int KT>
-__device__ __forceinline__ bool tree_whole(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob& t) {
-    const int lin = blockIdx.x, y = lin / 8, w = (y / p.row_blocks) * 8 + lin % 8;     // (as tree_next)
-    t.kh = w % c.n_kv_head; t.rb = y % p.row_blocks; t.i = t.w = w / c.n_kv_head; t.whole = 1; t.piece = 0; t.takers = 0; t.last = 1;
+__device__ __forceinline__ bool tree_whole(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob& t, int solo) {
+    const int lin = blockIdx.x, y = lin / 8, w = solo < 0 ? (y / p.row_blocks) * 8 + lin % 8 : 4 * lin + solo;     // (as tree_next)
+    t.kh = w % c.n_kv_head; t.rb = solo < 0 ? y % p.row_blocks : 0; t.i = t.w = w / c.n_kv_head; t.whole = 1; t.piece = 0; t.takers = 0; t.last = 1;
     t.all = t.start = t.x0 = t.x1 = 0;
     if (t.w >= p.slots) return false;
     tree_fill(c, a, p, KT, t);
     t.t0 = 0; t.t1 = t.n_pre + p.tree_tiles;
     return true;
 }
-// A job's second look, by all threads of the workgroup, each with its share of it: whether a page of the piece's tiles is none of the
+// A job's second look, by all threads that work on it, each with its share of it: whether a page of the piece's tiles is none of the
 // pool's, a page of the draft's rows is not this slot's alone although they are to be written, or an appending call names the slot
 // before.  What comes of it is needed at the end only (nothing is written before, and page_ok() keeps the reads inside the pool), so that
 // its loads overlap the work.
-__device__ __forceinline__ int tree_bad(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, int kt) {
+__device__ __forceinline__ int tree_bad(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, int kt, int me, int threads) {
     int bad = 0;
     const int32_t* row = c.d_table + (int64_t)j.seq * c.max_pages;
     const int upto = j.t1 > j.n_pre ? j.len + j.count : min(j.len, j.t1 * kt);
     const int own = a.d_kn && j.last ? j.len >> p.shift : 0x7fffffff;
-    for (int q = (min(j.t0 * kt, j.len) >> p.shift) + threadIdx.x; q << p.shift < upto; q += blockDim.x) {
+    for (int q = (min(j.t0 * kt, j.len) >> p.shift) + me; q << p.shift < upto; q += threads) {
         const int page = row[q];
         if ((unsigned)page >= (unsigned)c.n_pages || (q >= own && c.d_refs[page] != 1)) bad = 1;
     }
-    if (a.d_kn) for (int k = threadIdx.x; k < j.i; k += blockDim.x) bad |= a.d_seqs[k] == j.seq;
+    if (a.d_kn) for (int k = me; k < j.i; k += threads) bad |= a.d_seqs[k] == j.seq;
     return bad;
 }
 __device__ __forceinline__ int page_ok(const wx_cache& c, int page) { return (unsigned)page < (unsigned)c.n_pages ? page : 0; }
@@ -391,9 +391,9 @@ __device__ __forceinline__ T* append_place(const wx_cache& c, const TreePlan& p,
     return reinterpret_cast<T*>(u < j.count * PER ? c.d_k : c.d_v) + head_off + page_ok(c, table[t >> p.shift]) * page_e + (int64_t)(t & (c.page_size - 1)) * D + x * E;
 }
 template <typename T, int D>
-__device__ __forceinline__ void append_nodes(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off, int64_t page_e, int u0) {
+__device__ __forceinline__ void append_nodes(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, const TreeJob& j, const int32_t* table, int64_t head_off, int64_t page_e, int u0, int threads) {
     constexpr int PER = D * (int)sizeof(T) / 16;
-    for (int u = u0; u < j.count * PER * 2; u += blockDim.x) *reinterpret_cast<i32x4*>(append_place<T, D>(c, p, j, table, head_off, page_e, u)) = append_load<T, D>(c, a, j, u);
+    for (int u = u0; u < j.count * PER * 2; u += threads) *reinterpret_cast<i32x4*>(append_place<T, D>(c, p, j, table, head_off, page_e, u)) = append_load<T, D>(c, a, j, u);
 }
 
 template <typename T> __device__ __forceinline__ void store4(T* to, f32x4 v);
@@ -410,27 +410,32 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // values (through the wave's own LDS, for the transposing read); the next tile's 16 loads a lane are issued as soon as the scores of
 // this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
 // Against one thread a key and head, without matrix instructions: 16 x 24 rows, 20 heads of 64, 30-420 tokens: 268 us -> 15 us (24 MB;
-// latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us (111 MB, 3.5 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
+// latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us, 29 SOLO (111 MB, 3.8 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
 // With three waves a SIMD instead of two the registers spill and 64 x 1 row take 33 us.
-template <typename T, int D, int RT, bool ONE>
+// SOLO (whole sequences, up to 16 rows, jobs enough to fill the chip: tree_solo): every wave has a job of its own and takes all of its tiles, so
+// that all jobs are under way at once and nothing is merged.
+template <typename T, int D, int RT, bool ONE, bool SOLO = false>
 __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
+    static_assert(!SOLO || (ONE && RT == 1), "a wave alone does one whole sequence");
+    constexpr int STEP = SOLO ? 1 : 4, THREADS = SOLO ? 64 : 256;
     typedef typename Elem<T>::Frag Frag;
     constexpr int E = 16 / sizeof(T), KT = 8192 / (D * (int)sizeof(T)), NS = KT / 16, KS = D / (4 * E), CPR = D / E, NV = KT * CPR / 64;
     constexpr int VROW = D * (int)sizeof(T) + Elem<T>::PAD, VBYTES = KT * VROW, OROW = 68;
-    constexpr int LDS = 4 * VBYTES > 4 * RT * 16 * OROW * 4 ? 4 * VBYTES : 4 * RT * 16 * OROW * 4;
+    constexpr int LDS = SOLO || 4 * VBYTES > 4 * RT * 16 * OROW * 4 ? 4 * VBYTES : 4 * RT * 16 * OROW * 4;
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     __shared__ TreeJob s_job;
     __shared__ int s_wrong[64];
     __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
-    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15, me = SOLO ? lane : tid;
     TreeJob j;
     for (bool first = true;; first = false) {
     TREE_ARGS(ka);
-    if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j)) break; }
+    if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j, SOLO ? wid : -1)) break; }
     else if (!tree_next<KT>(c, a, p, &s_job, j, first)) break;
     tree_uniform(j);
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * RT * 16;
     int bad = 0;
+    bool row_wrong = false;
     const bool writes = j.ok == 1 && a.d_kn && j.rb == 0 && j.last;
     i32x4 row0_part = {0, 0, 0, 0};
     T* place = nullptr;
@@ -519,7 +524,8 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
         // on their way while the length and the pages are looked up.  Every lane has the mask of its node and takes those of its rows.
         bool wrong = a.d_parents && a.n_nodes == 1 && a.d_parents[j.i] != -1;
         const uint64_t own_mask = a.n_nodes == 1 ? 1 : tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
-        if (wid == 0) s_wrong[lane] = wrong;
+        if constexpr (SOLO) row_wrong = __shfl((int)wrong, min(row0 + r, rows - 1) / G);
+        else if (wid == 0) s_wrong[lane] = wrong;
         uint64_t mask[RT];
 #pragma unroll
         for (int q = 0; q < RT; ++q) {
@@ -527,7 +533,7 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
             mask[q] = (uint64_t)(uint32_t)__shfl((uint32_t)(own_mask >> 32), node) << 32 | (uint32_t)__shfl((uint32_t)own_mask, node);
         }
         const int nt0 = ONE ? 0 : max(0, j.t0 - j.n_pre), nt1 = ONE ? p.tree_tiles : j.t1 - j.n_pre;
-        for (int nt = nt0 + 3 - wid; nt < nt1; nt += 4) {
+        for (int nt = nt0 + (SOLO ? 0 : 3 - wid); nt < nt1; nt += STEP) {
             const int node0 = nt * KT;
             if (node0 >= j.count) break;
             f32x4 s[NS][RT];
@@ -553,22 +559,22 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
             __builtin_amdgcn_wave_barrier();
         }
         const int end = min(j.t1, j.n_pre);
-        int t = j.t0 + wid;
-        if (writes && tid < j.count * CPR * 2) { row0_part = append_load<T, D>(c, a, j, tid); place = append_place<T, D>(c, p, j, table, head_off, page_e, tid); }
-        if (t >= end) bad = tree_bad(c, a, p, j, KT);
+        int t = j.t0 + (SOLO ? 0 : wid);
+        if (writes && me < j.count * CPR * 2) { row0_part = append_load<T, D>(c, a, j, me); place = append_place<T, D>(c, p, j, table, head_off, page_e, me); }
+        if (t >= end) bad = tree_bad(c, a, p, j, KT, me, THREADS);
         else {
             int ids = load_ids(t);
             load_pre(t, ids);
-            ids = load_ids(min(t + 4, j.n_pre - 1));
-            bad = tree_bad(c, a, p, j, KT);
-            for (; t < end; t += 4) {
+            ids = load_ids(min(t + STEP, j.n_pre - 1));
+            bad = tree_bad(c, a, p, j, KT, me, THREADS);
+            for (; t < end; t += STEP) {
                 f32x4 s[NS][RT];
                 const int live = j.len - t * KT;
                 stage(live);
                 scores(s);
-                if (t + 4 < end) {
-                    load_pre(t + 4, ids);
-                    ids = load_ids(min(t + 8, j.n_pre - 1));
+                if (t + STEP < end) {
+                    load_pre(t + STEP, ids);
+                    ids = load_ids(min(t + 2 * STEP, j.n_pre - 1));
                 }
                 if (live < KT) {
                     asm volatile("");                                               // keep it a branch: as selects it costs every tile
@@ -586,6 +592,25 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
             }
         }
     }
+    if constexpr (SOLO) {
+        if (__builtin_amdgcn_ballot_w64(bad != 0)) j.ok = 2;
+        if (writes && j.ok == 1) {
+            if (me < j.count * CPR * 2) *reinterpret_cast<i32x4*>(place) = row0_part;
+            append_nodes<T, D>(c, a, p, j, table, head_off, page_e, me + THREADS, THREADS);
+        }
+        float l = st.l[0];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        const int node = r / G;
+        if (r < rows) {
+            T* out = reinterpret_cast<T*>(a.d_out) + j.i * a.o_seq + node * a.o_node + (j.kh * G + r % G) * a.o_head + 4 * g;
+            const int kind = j.ok == 1 ? node >= j.count ? 0 : row_wrong ? 2 : 1 : j.ok;
+            const float f = 1.f / l;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) store4<T>(out + 16 * d, kind == 1 ? st.o[d][0] * f : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
+        }
+        break;
+    }
     // ---- the four waves' states: factors first, then 64 columns of the outputs at a time ---------------------------------------------
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -596,8 +621,8 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
     }
     if (__builtin_amdgcn_readfirstlane(__syncthreads_or(bad))) j.ok = 2;
     if (writes && j.ok == 1) {
-        if (tid < j.count * CPR * 2) *reinterpret_cast<i32x4*>(place) = row0_part;
-        append_nodes<T, D>(c, a, p, j, table, head_off, page_e, tid + 256);
+        if (me < j.count * CPR * 2) *reinterpret_cast<i32x4*>(place) = row0_part;
+        append_nodes<T, D>(c, a, p, j, table, head_off, page_e, me + THREADS, THREADS);
     }
     const bool whole = j.whole;
     float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (RT * 16) * (D + 2);
@@ -690,7 +715,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     TreeJob j;
     for (bool first = true;; first = false) {
     TREE_ARGS(ka);
-    if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j)) break; }
+    if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j, -1)) break; }
     else if (!tree_next<KT>(c, a, p, &s_job, j, first)) break;
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, part_row0 = ((wid & 3) * 2 + (wid >> 2)) * 16 * RT, row0 = j.rb * TRW * 16 * RT + part_row0;
     if (wid == 0 && j.ok == 1) {
@@ -700,7 +725,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     }
     if (tid == 0) { s_bad = 0; if (ONE) s_job = j; }
     __syncthreads();
-    if (j.ok == 1 && tree_bad(c, a, p, j, KT)) s_bad = 1;                          // (read behind later barriers)
+    if (j.ok == 1 && tree_bad(c, a, p, j, KT, tid, 64 * TRW)) s_bad = 1;                          // (read behind later barriers)
     const int seq = __builtin_amdgcn_readfirstlane(j.seq), kh = __builtin_amdgcn_readfirstlane(j.kh), len = __builtin_amdgcn_readfirstlane(j.len);
     const int32_t* table = c.d_table + (int64_t)seq * c.max_pages;
     const int64_t page_e = (int64_t)c.n_kv_head * c.page_size * D, head_off = (int64_t)a.layer * c.n_pages * page_e + (int64_t)kh * c.page_size * D;
@@ -942,7 +967,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     __syncthreads();
     j = s_job;
     if (j.ok == 1 && s_bad) j.ok = 2;
-    if (j.ok == 1 && a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e, tid);
+    if (j.ok == 1 && a.d_kn && j.rb == 0 && j.last) append_nodes<T, D>(c, a, p, j, table, head_off, page_e, tid, 64 * TRW);
     const bool whole = j.whole;
     float* part = whole ? nullptr : p.part + (((int64_t)j.piece * c.n_kv_head + j.kh) * p.row_blocks + j.rb) * (TRW * 16 * RT) * (D + 2);
 #pragma unroll
@@ -1130,6 +1155,15 @@ static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeFo
     p.merge_rows = 1024 / c.head_dim;
     while (p.merge_rows > 1 && merges * ((rows + p.merge_rows / 2 - 1) / (p.merge_rows / 2)) <= 2048 * (int64_t)p.row_blocks) p.merge_rows /= 2;
     return p;
+}
+// Whether a wave alone takes a whole sequence (a key / value head's up to 16 rows): jobs enough to fill the chip without cutting them, and
+// few tiles each.  us with four waves a job / one, 20 heads, 1 row: bf16, heads of 64, 200-447 tokens: 40 sequences 21.0 / 20.4, 64 30.6 / 29.4, 100
+// 40.9 / 33.8, 200 89.5 / 70.5; 20-100 tokens: 40 15.2 / 12.2, 64 19.8 / 14.4, 200 53.9 / 27.4; f32, 64, 20-100: 26 15.2 / 16.9, 40 17.9 / 17.7, 200
+// 64.6 / 40.5.  More tiles (bf16, heads of 128, 447 tokens: 15): 64 42.7 / 46.1, 100 68.0 / 62.9; 29 tiles (f32): 200 247 / 264.  With
+// split_tokens a result must not depend on the number of sequences.
+static bool tree_solo(const wx_cache& c, const wx_tree_attn& a, const TreeForm& f, const TreePlan& p) {
+    const int64_t jobs = (int64_t)a.n * c.n_kv_head, most = ((int64_t)c.max_pages * c.page_size + f.kt - 1) / f.kt + p.tree_tiles;
+    return p.single && a.split_tokens == 0 && a.n_nodes * (a.n_head / c.n_kv_head) <= 16 && ((jobs >= 768 && most <= 9) || (jobs >= 2000 && most <= 16));
 }
 static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {
     return (int64_t)p.pieces * c.n_kv_head * p.row_blocks * p.rows * (c.head_dim + 2) * 4;
@@ -1342,6 +1376,7 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
     if (jobs > 0x7fffff) return set_error(WX_ERR_INVALID, "too many pieces of work: fewer sequences, or larger split_tokens");
     const dim3 grid((unsigned)jobs), block(256);
     const bool f32 = c->precision == WX_PREC_F32, wide = c->head_dim == 128;
+#define TREE_SOLO(T, D) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, 1, true, true>), dim3((unsigned)((jobs + 3) / 4)), block, 0, st, TreeArgs{*c, *a, p})
 #define TREE_KEYS(T, D, RT) do { if (p.single) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, true>), grid, block, 0, st, TreeArgs{*c, *a, p}); \
                                  else hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, false>), grid, block, 0, st, TreeArgs{*c, *a, p}); } while (0)
 #define TREE_ROWS(D, RT) do { const int lds = 4 * 2 * 64 * D * 2; \
@@ -1350,6 +1385,9 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
     if (f.rows_form) {
         if (wide) { if (f.rt == 2) TREE_ROWS(128, 2); else TREE_ROWS(128, 1); }
         else TREE_ROWS(64, 2);
+    } else if (tree_solo(*c, *a, f, p)) {
+        if (f32) { if (wide) TREE_SOLO(float, 128); else TREE_SOLO(float, 64); }
+        else { if (wide) TREE_SOLO(bf16, 128); else TREE_SOLO(bf16, 64); }
     } else if (f32) {
         if (wide) TREE_KEYS(float, 128, 1);
         else { if (f.rt == 2) TREE_KEYS(float, 64, 2); else TREE_KEYS(float, 64, 1); }
