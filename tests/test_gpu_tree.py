@@ -104,7 +104,7 @@ def test_against_64_bits(dtype, lens, N, heads, kv_heads, D, PS, append):
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
 @pytest.mark.parametrize("n,N,heads,kv_heads,D,longest", [(130, 1, 8, 8, 64, 500), (129, 5, 24, 8, 64, 90), (66, 16, 16, 16, 128, 140), (1100, 1, 4, 1, 64, 33), (35, 2, 60, 30, 128, 508),
-                                                          (70, 3, 24, 12, 128, 60)])
+                                                          (70, 3, 24, 12, 128, 60), (50, 20, 32, 8, 64, 60), (48, 24, 20, 20, 64, 400), (400, 33, 2, 1, 64, 20)])
 def test_many_short_sequences(dtype, n, N, heads, kv_heads, D, longest):
     """more sequences x heads than waves fit at once, short enough for a wave each: ragged, some empty, some padding, some refused"""
     rng = np.random.RandomState(n + N)

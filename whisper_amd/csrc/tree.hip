@@ -168,8 +168,8 @@ __device__ __forceinline__ void tree_uniform(TreeJob& t) {
 // The one job of a workgroup that does one whole sequence, or (solo >= 0) of its wave `solo`: no search, and nothing waits for another wave.
 template <int KT>
 __device__ __forceinline__ bool tree_whole(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, TreeJob& t, int solo) {
-    const int lin = blockIdx.x, y = lin / 8, w = solo < 0 ? (y / p.row_blocks) * 8 + lin % 8 : 4 * lin + solo;     // (as tree_next)
-    t.kh = w % c.n_kv_head; t.rb = solo < 0 ? y % p.row_blocks : 0; t.i = t.w = w / c.n_kv_head; t.whole = 1; t.piece = 0; t.takers = 0; t.last = 1;
+    const int lin = blockIdx.x, y = lin / 8, w = solo < 0 ? (y / p.row_blocks) * 8 + lin % 8 : (4 * lin + solo) / p.row_blocks;     // (as tree_next)
+    t.kh = w % c.n_kv_head; t.rb = (solo < 0 ? y : 4 * lin + solo) % p.row_blocks; t.i = t.w = w / c.n_kv_head; t.whole = 1; t.piece = 0; t.takers = 0; t.last = 1;
     t.all = t.start = t.x0 = t.x1 = 0;
     if (t.w >= p.slots) return false;
     tree_fill(c, a, p, KT, t);
@@ -412,11 +412,11 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // Against one thread a key and head, without matrix instructions: 16 x 24 rows, 20 heads of 64, 30-420 tokens: 268 us -> 15 us (24 MB;
 // latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us, 29 SOLO (111 MB, 3.8 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
 // With three waves a SIMD instead of two the registers spill and 64 x 1 row take 33 us.
-// SOLO (whole sequences, up to 16 rows, jobs enough to fill the chip: tree_solo): every wave has a job of its own and takes all of its tiles, so
+// SOLO (whole sequences, jobs enough to fill the chip: tree_solo): every wave has a job of its own and takes all of its tiles, so
 // that all jobs are under way at once and nothing is merged.
 template <typename T, int D, int RT, bool ONE, bool SOLO = false>
 __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
-    static_assert(!SOLO || (ONE && RT == 1), "a wave alone does one whole sequence");
+    static_assert(!SOLO || ONE, "a wave alone does one whole sequence");
     constexpr int STEP = SOLO ? 1 : 4, THREADS = SOLO ? 64 : 256;
     typedef typename Elem<T>::Frag Frag;
     constexpr int E = 16 / sizeof(T), KT = 8192 / (D * (int)sizeof(T)), NS = KT / 16, KS = D / (4 * E), CPR = D / E, NV = KT * CPR / 64;
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
     tree_uniform(j);
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, row0 = j.rb * RT * 16;
     int bad = 0;
-    bool row_wrong = false;
+    bool row_wrong[RT] = {};
     const bool writes = j.ok == 1 && a.d_kn && j.rb == 0 && j.last;
     i32x4 row0_part = {0, 0, 0, 0};
     T* place = nullptr;
@@ -524,13 +524,13 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
         // on their way while the length and the pages are looked up.  Every lane has the mask of its node and takes those of its rows.
         bool wrong = a.d_parents && a.n_nodes == 1 && a.d_parents[j.i] != -1;
         const uint64_t own_mask = a.n_nodes == 1 ? 1 : tree_mask(a.d_parents ? a.d_parents + (int64_t)j.i * a.n_nodes : nullptr, lane, a.n_nodes, &wrong);
-        if constexpr (SOLO) row_wrong = __shfl((int)wrong, min(row0 + r, rows - 1) / G);
-        else if (wid == 0) s_wrong[lane] = wrong;
+        if (!SOLO && wid == 0) s_wrong[lane] = wrong;
         uint64_t mask[RT];
 #pragma unroll
         for (int q = 0; q < RT; ++q) {
             const int node = min(row0 + q * 16 + r, rows - 1) / G;
             mask[q] = (uint64_t)(uint32_t)__shfl((uint32_t)(own_mask >> 32), node) << 32 | (uint32_t)__shfl((uint32_t)own_mask, node);
+            if constexpr (SOLO) row_wrong[q] = __shfl((int)wrong, node);
         }
         const int nt0 = ONE ? 0 : max(0, j.t0 - j.n_pre), nt1 = ONE ? p.tree_tiles : j.t1 - j.n_pre;
         for (int nt = nt0 + (SOLO ? 0 : 3 - wid); nt < nt1; nt += STEP) {
@@ -598,16 +598,18 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
             if (me < j.count * CPR * 2) *reinterpret_cast<i32x4*>(place) = row0_part;
             append_nodes<T, D>(c, a, p, j, table, head_off, page_e, me + THREADS, THREADS);
         }
-        float l = st.l[0];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        const int node = r / G;
-        if (r < rows) {
-            T* out = reinterpret_cast<T*>(a.d_out) + j.i * a.o_seq + node * a.o_node + (j.kh * G + r % G) * a.o_head + 4 * g;
-            const int kind = j.ok == 1 ? node >= j.count ? 0 : row_wrong ? 2 : 1 : j.ok;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float l = st.l[t];
+            l += __shfl_xor(l, 16);
+            l += __shfl_xor(l, 32);
+            const int at = row0 + t * 16 + r, node = at / G;
+            if (at >= rows) continue;
+            T* out = reinterpret_cast<T*>(a.d_out) + j.i * a.o_seq + node * a.o_node + (j.kh * G + at % G) * a.o_head + 4 * g;
+            const int kind = j.ok == 1 ? node >= j.count ? 0 : row_wrong[t] ? 2 : 1 : j.ok;
             const float f = 1.f / l;
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) store4<T>(out + 16 * d, kind == 1 ? st.o[d][0] * f : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
+            for (int d = 0; d < D / 16; ++d) store4<T>(out + 16 * d, kind == 1 ? st.o[d][t] * f : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
         }
         break;
     }
@@ -1156,14 +1158,16 @@ static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeFo
     while (p.merge_rows > 1 && merges * ((rows + p.merge_rows / 2 - 1) / (p.merge_rows / 2)) <= 2048 * (int64_t)p.row_blocks) p.merge_rows /= 2;
     return p;
 }
-// Whether a wave alone takes a whole sequence (a key / value head's up to 16 rows): jobs enough to fill the chip without cutting them, and
+// Whether a wave alone takes a whole sequence (a key / value head, a block of rows): jobs enough to fill the chip without cutting them, and
 // few tiles each.  us with four waves a job / one, 20 heads, 1 row: bf16, heads of 64, 200-447 tokens: 40 sequences 21.0 / 20.4, 64 30.6 / 29.4, 100
 // 40.9 / 33.8, 200 89.5 / 70.5; 20-100 tokens: 40 15.2 / 12.2, 64 19.8 / 14.4, 200 53.9 / 27.4; f32, 64, 20-100: 26 15.2 / 16.9, 40 17.9 / 17.7, 200
-// 64.6 / 40.5.  More tiles (bf16, heads of 128, 447 tokens: 15): 64 42.7 / 46.1, 100 68.0 / 62.9; 29 tiles (f32): 200 247 / 264.  With
-// split_tokens a result must not depend on the number of sequences.
+// 64.6 / 40.5.  More tiles (bf16, heads of 128, 447 tokens: 15): 64 42.7 / 46.1, 100 68.0 / 62.9; 29 tiles (f32): 200 247 / 264.  More rows, bf16:
+// 64 x 92 rows, 8 heads, 5-9 tokens 29.6 / 16.1, 64 x 24, 20 heads, 30-420 tokens 36.6 / 32.6; f32, whose products take longer: 40 x 24, 20 heads,
+// 30-420 tokens 51 / 59.  With split_tokens a result must not depend on the number of sequences.
 static bool tree_solo(const wx_cache& c, const wx_tree_attn& a, const TreeForm& f, const TreePlan& p) {
-    const int64_t jobs = (int64_t)a.n * c.n_kv_head, most = ((int64_t)c.max_pages * c.page_size + f.kt - 1) / f.kt + p.tree_tiles;
-    return p.single && a.split_tokens == 0 && a.n_nodes * (a.n_head / c.n_kv_head) <= 16 && ((jobs >= 768 && most <= 9) || (jobs >= 2000 && most <= 16));
+    const int rows = a.n_nodes * (a.n_head / c.n_kv_head);
+    const int64_t jobs = (int64_t)a.n * c.n_kv_head * p.row_blocks, most = ((int64_t)c.max_pages * c.page_size + f.kt - 1) / f.kt + p.tree_tiles;
+    return p.single && a.split_tokens == 0 && !f.rows_form && (c.precision == WX_PREC_BF16 || rows <= 16) && ((jobs >= 768 && most <= 9) || (jobs >= 2000 && most <= 16));
 }
 static int64_t tree_part_bytes(const wx_cache& c, const TreePlan& p) {
     return (int64_t)p.pieces * c.n_kv_head * p.row_blocks * p.rows * (c.head_dim + 2) * 4;
@@ -1376,7 +1380,7 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
     if (jobs > 0x7fffff) return set_error(WX_ERR_INVALID, "too many pieces of work: fewer sequences, or larger split_tokens");
     const dim3 grid((unsigned)jobs), block(256);
     const bool f32 = c->precision == WX_PREC_F32, wide = c->head_dim == 128;
-#define TREE_SOLO(T, D) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, 1, true, true>), dim3((unsigned)((jobs + 3) / 4)), block, 0, st, TreeArgs{*c, *a, p})
+#define TREE_SOLO(T, D, RT) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, true, true>), dim3((unsigned)((jobs + 3) / 4)), block, 0, st, TreeArgs{*c, *a, p})
 #define TREE_KEYS(T, D, RT) do { if (p.single) hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, true>), grid, block, 0, st, TreeArgs{*c, *a, p}); \
                                  else hipLaunchKernelGGL((tree_attention_keys_kernel<T, D, RT, false>), grid, block, 0, st, TreeArgs{*c, *a, p}); } while (0)
 #define TREE_ROWS(D, RT) do { const int lds = 4 * 2 * 64 * D * 2; \
@@ -1386,8 +1390,8 @@ int wx_tree_attention(const wx_cache* c, const wx_tree_attn* a, void* stream) {
         if (wide) { if (f.rt == 2) TREE_ROWS(128, 2); else TREE_ROWS(128, 1); }
         else TREE_ROWS(64, 2);
     } else if (tree_solo(*c, *a, f, p)) {
-        if (f32) { if (wide) TREE_SOLO(float, 128); else TREE_SOLO(float, 64); }
-        else { if (wide) TREE_SOLO(bf16, 128); else TREE_SOLO(bf16, 64); }
+        if (f32) { if (wide) TREE_SOLO(float, 128, 1); else TREE_SOLO(float, 64, 1); }
+        else { if (wide) TREE_SOLO(bf16, 128, 1); else if (f.rt == 2) TREE_SOLO(bf16, 64, 2); else TREE_SOLO(bf16, 64, 1); }
     } else if (f32) {
         if (wide) TREE_KEYS(float, 128, 1);
         else { if (f.rt == 2) TREE_KEYS(float, 64, 2); else TREE_KEYS(float, 64, 1); }
