@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void cache_copy_tail_kernel(PageArgs a) {
 // ---- append: grid (entry, group of AP_NODES nodes, group of layers) -------------------------------------------------------------------
 // The entry is checked and its places are looked up once for all layers of the group; a thread then takes its 16 bytes of keys and of
 // values through the layers, two layers' loads at a time.  Bound by the copy: 64 x 16 rows (769 there), 32 layers x 20 heads of 64: 252 MB in
-// 55 us, 4.6 TB/s.
+// 52 us, 4.8 TB/s; 16 x 24 rows, 4 layers: 7 us (latency).
 constexpr int AP_NODES = 4;
 __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs b) {
     __shared__ int64_t place[AP_NODES];
@@ -355,7 +355,7 @@ __device__ __forceinline__ bool commit_ok(const PageArgs& a, int i, int* taken, 
 // grid (entry, group of layers): a thread takes 16 bytes of a head's rows of one layer, keys or values, down the whole path.  path[k] >= k
 // and ascends, so a row that is overwritten was read before by the same thread (eight rows are read before they are written); rows that
 // stay (path[k] == k) are not touched.  Where one group holds all layers, the workgroup sets the length itself (saves a launch: 4.7 us).
-// 64 entries, 32 layers x 20 heads of 64, 241 rows taken: 38 MB in 15 us; 16 entries, 4 layers: 9.7 us (latency: a page number, then rows).
+// 64 entries, 32 layers x 20 heads of 64, 241 rows taken: 38 MB in 13 us; 16 entries, 4 layers: 8.6 us (latency).
 constexpr int CM_ROWS = 64;                                          // moves looked up at a time
 __global__ __launch_bounds__(256) void cache_commit_rows_kernel(PageArgs a) {
     __shared__ int64_t from[CM_ROWS], to[CM_ROWS];

@@ -410,7 +410,7 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // values (through the wave's own LDS, for the transposing read); the next tile's 16 loads a lane are issued as soon as the scores of
 // this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
 // Against one thread a key and head, without matrix instructions: 16 x 24 rows, 20 heads of 64, 30-420 tokens: 268 us -> 15 us (24 MB;
-// latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us, 29 SOLO (111 MB, 3.8 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
+// latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us, 29 with SOLO (111 MB, 3.8 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
 // With three waves a SIMD instead of two the registers spill and 64 x 1 row take 33 us.
 // SOLO (whole sequences, jobs enough to fill the chip: tree_solo): every wave has a job of its own and takes all of its tiles, so
 // that all jobs are under way at once and nothing is merged.
@@ -1301,7 +1301,7 @@ __global__ __launch_bounds__(64) void tree_verify_walk_kernel(wx_tree_check a, i
     if (j < count) {
         Best b{-INFINITY, 0.f, 0x7fffffff};
         const f32x4* rec = reinterpret_cast<const f32x4*>(a.d_work) + ((int64_t)i * a.n_nodes + j) * parts;
-#pragma unroll 4
+#pragma unroll 8
         for (int p = 0; p < parts; ++p) { const f32x4 x = rec[p]; b = best_merge(b, Best{x[0], x[1], __builtin_bit_cast(int, (float)x[2])}); }
         pick = b.m > -INFINITY ? b.i : -1;
         lp = b.m > -INFINITY ? -logf(b.s) : -INFINITY;
