@@ -58,6 +58,12 @@ struct TreeArgs { wx_cache c; wx_tree_attn a; TreePlan p; };
     const wx_tree_attn& a = ((const TreeArgs*)ka##_p)->a; \
     const TreePlan& p = ((const TreeArgs*)ka##_p)->p
 
+// So is the thread's number: addresses that follow from it would be kept over the loop of jobs as well, 20 to 30 vector registers of them, and
+// push some to scratch memory.
+#define TREE_THREAD(tid) \
+    int tid = threadIdx.x; \
+    asm volatile("" : "+v"(tid))
+
 // What a workgroup has to do now: sequence entry i, key / value head, block of rows, tiles [t0, t1) of the sequence's n_pre + tree_tiles.
 struct TreeJob {
     int ok;                  // 0: the rows are 0 (padding, no nodes), 1: attend, 2: refused (NaN), -1: nothing (any more)
@@ -411,7 +417,8 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
 // Against one thread a key and head, without matrix instructions: 16 x 24 rows, 20 heads of 64, 30-420 tokens: 268 us -> 15 us (24 MB;
 // latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us, 29 with SOLO (111 MB, 3.8 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
-// With three waves a SIMD instead of two the registers spill and 64 x 1 row take 33 us.
+// With three waves a SIMD instead of two the vector registers spill, 64 x 1 row take 33 us, and the cut form of that build gave wrong results (cause not
+// established): no kernel here keeps vector registers in scratch memory.
 // SOLO (whole sequences, jobs enough to fill the chip: tree_solo): every wave has a job of its own and takes all of its tiles, so
 // that all jobs are under way at once and nothing is merged.
 template <typename T, int D, int RT, bool ONE, bool SOLO = false>
@@ -426,10 +433,11 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
     __shared__ TreeJob s_job;
     __shared__ int s_wrong[64];
     __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
-    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15, me = SOLO ? lane : tid;
     TreeJob j;
     for (bool first = true;; first = false) {
     TREE_ARGS(ka);
+    TREE_THREAD(tid);
+    const int lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15, me = SOLO ? lane : tid;
     if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j, SOLO ? wid : -1)) break; }
     else if (!tree_next<KT>(c, a, p, &s_job, j, first)) break;
     tree_uniform(j);
@@ -712,11 +720,12 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
     __shared__ TreeJob s_job;
     __shared__ uint64_t s_mask[64];
     __shared__ int s_wrong[64], s_bad;
-    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
-    const bool late = wid >= TRW / 2;
     TreeJob j;
     for (bool first = true;; first = false) {
     TREE_ARGS(ka);
+    TREE_THREAD(tid);
+    const int lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
+    const bool late = wid >= TRW / 2;
     if constexpr (ONE) { if (!first || !tree_whole<KT>(c, a, p, j, -1)) break; }
     else if (!tree_next<KT>(c, a, p, &s_job, j, first)) break;
     const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, part_row0 = ((wid & 3) * 2 + (wid >> 2)) * 16 * RT, row0 = j.rb * TRW * 16 * RT + part_row0;
