@@ -295,8 +295,8 @@ int wx_cache_compact(const wx_cache* c, int32_t* d_n_live, void* stream);
  * call (as wx_cache_append does; the ids must be distinct then), without (both NULL) they lie there.  A sequence id out of range, rows that are not reserved or
  * whose pages another slot holds too, and a second entry of the same id in an appending call give rows of NaN and append nothing.  The
  * rows of a sequence with a page number outside the pool, and of a node with a parent out of range and its descendants, are NaN as well.  n_nodes == 1 is the ordinary decode step.  n_head: query heads, a multiple of n_kv_head up to 16 x as many; head h reads key/value head
- * h / (n_head / n_kv_head).  Strides in elements: heads' rows are contiguous and 16-byte aligned.  Softmax and sums in fp32; bf16
- * caches round the probabilities to bf16 for the product with the values.  What masked rows hold (NaN, infinities) has no effect.
+ * h / (n_head / n_kv_head).  Strides in elements: heads' rows are contiguous and 16-byte aligned.  Softmax and sums in fp32; on bf16
+ * caches the probabilities enter the product with the values as two bf16 numbers each (16 bits).  What masked rows hold (NaN, infinities) has no effect.
  * split_tokens: the committed tokens are cut into pieces that workgroups take side by side; 0 = by the size of the batch; > 0 = pieces
  * of that many tokens (rounded up to a tile of 16 to 64 tokens, and to a 256th of what a table holds), so that a sequence's result does
  * not depend on what else is in the batch.  d_out may be d_q. */

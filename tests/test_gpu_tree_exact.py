@@ -1,0 +1,86 @@
+"""Tree attention of bf16 caches held to what the rounding of its result alone allows: probabilities keep their bits, and no key is lost
+wherever it stands."""
+import numpy as np
+import pytest
+import torch
+
+import kv_model as km
+from test_gpu_tree import BF16, Case, i32
+
+pytestmark = pytest.mark.gpu
+
+
+def tight_bound(o, mass, reach, D, tokens):
+    """kv_model.attention_bound for 32 bits (scores, exponentials and sums; a probability enters as two bf16 terms, so there are twice as many
+    additions), 2^-14 of every probability for what two bf16 terms leave out (half a step, 2^-8, of a second term of at most 2^-7 + 2^-8 of it), and
+    half a step, 2^-8, of the result."""
+    u = 2.0 ** -24
+    rel = 2 * (D + 4) * u * reach + (4 * tokens + 64) * u + 2.0 ** -14
+    return rel * mass * (1 + 2.0 ** -7) + 2.0 ** -8 * np.abs(o) + 1e-30
+
+
+def check(c, out, scale=None):
+    scale = c.D ** -0.5 if scale is None else scale
+    out = out.float().cpu().numpy().astype(np.float64)
+    for i in range(c.n):
+        K, V = torch.cat([c.pre[i][0], c.kn[i]]).float().numpy(), torch.cat([c.pre[i][1], c.vn[i]]).float().numpy()
+        o, mass, reach = km.tree_attention(c.q[i].float().numpy(), K, V, c.par[i], scale)
+        off, bound = np.abs(out[i] - o), tight_bound(o, mass, reach, c.D, len(K))
+        assert (off <= bound).all(), (i, float((off / bound).max()), int((off > bound).sum()))
+
+
+# every kernel for bf16 caches: the waves share the keys (16 or 32 rows; a whole sequence or pieces), a wave alone, the waves share the rows
+@pytest.mark.parametrize("lens,N,heads,kv_heads,D,PS", [
+    ([30, 100], 5, 4, 2, 64, 16), ([90, 200], 24, 3, 3, 64, 16), ([64, 9], 6, 4, 2, 128, 16), ([700, 20], 5, 4, 2, 64, 16), ([700, 90], 24, 3, 3, 64, 16),
+    ([600, 31], 6, 4, 2, 128, 32), (list(range(0, 130)), 1, 8, 8, 64, 16), (list(range(3, 100)), 2, 16, 8, 128, 16), (list(range(1, 65)), 20, 12, 12, 64, 16),
+    ([50, 129], 40, 2, 2, 128, 16), ([65, 200], 40, 8, 2, 128, 32), ([900], 20, 4, 4, 128, 32), ([1000, 30], 64, 8, 2, 128, 64), ([40], 64, 16, 4, 64, 16), ([800, 3], 64, 6, 2, 64, 16)])
+def test_probabilities_keep_their_bits(lens, N, heads, kv_heads, D, PS):
+    c = Case(lens, N, heads, kv_heads, D, PS, BF16, seed=len(lens) + N)
+    c.q *= 3                                                       # the weight on few tokens, whose roundings do not average out
+    check(c, c.run())
+
+
+FORMS = [([30, 100], 5, 4, 2, 64, 16), ([90, 200], 24, 3, 3, 64, 16), ([64, 9], 6, 4, 2, 128, 16), ([700, 200], 5, 4, 2, 64, 16), ([700, 90], 24, 3, 3, 64, 16),
+         (list(range(20, 150)), 1, 8, 8, 64, 16), (list(range(20, 100)), 20, 12, 12, 64, 16), ([50, 129], 40, 2, 2, 128, 16), ([1000, 300], 64, 8, 2, 128, 64),
+         ([800, 30], 64, 6, 2, 64, 16)]
+
+
+@pytest.mark.parametrize("lens,N,heads,kv_heads,D,PS", FORMS)
+def test_infinite_values_of_committed_tokens(lens, N, heads, kv_heads, D, PS):
+    """every row attends them, so its column is infinite, with their sign; NaN where both signs meet, and nothing else changes"""
+    c = Case(lens, N, heads, kv_heads, D, PS, BF16, seed=1)
+    c.q *= 0.25                                                    # no probability is 0
+    clean = c.run().float().cpu()
+    for s in range(c.n):
+        for token, col, what in ((0, 3, float("inf")), (int(c.lens[s]) - 1, 17, -float("inf")), (int(c.lens[s]) // 2, 40, float("inf")), (1, 40, -float("inf"))):
+            page = int(c.cache.table[int(c.slots[s]), token // PS])
+            c.cache.v[c.layer, page, :, token % PS, col] = what
+    out = c.run().float().cpu()
+    assert (out[..., 3] == float("inf")).all() and (out[..., 17] == -float("inf")).all() and torch.isnan(out[..., 40]).all()
+    rest = [x for x in range(D) if x not in (3, 17, 40)]
+    assert torch.equal(out[..., rest], clean[..., rest])
+
+
+@pytest.mark.parametrize("lens,N,heads,kv_heads,D,PS", [
+    ([0, 1, 15, 16, 17, 31, 32, 33, 63, 64, 65], 24, 6, 2, 64, 16), ([447, 448, 129, 127], 64, 8, 1, 64, 16), ([511, 513, 640, 1000], 24, 16, 1, 64, 16),
+    ([128, 127, 129, 400], 12, 16, 2, 128, 32), ([575, 576, 577], 12, 16, 1, 128, 16), ([0, 1, 63, 64, 65, 127, 200], 17, 32, 2, 128, 16),
+    ([512, 511, 640, 2000], 64, 16, 1, 128, 64), ([700, 1023, 1025], 64, 15, 1, 64, 128), (list(range(100)), 3, 32, 8, 64, 16)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("split", [0, 64, 200])
+def test_no_key_is_lost(dtype, lens, N, heads, kv_heads, D, PS, split):
+    """every row points at one token, its own among those it attends, so that almost all of its weight is there: first, last and every other one of
+    the committed tokens (ends of tiles, pages, pieces and shares) in turn, and the node itself"""
+    c = Case(lens, N, heads, kv_heads, D, PS, dtype, seed=3)
+    G = heads // kv_heads
+    for s in range(c.n):
+        length = int(c.lens[s])
+        for node in range(N):
+            for h in range(heads):
+                at = (node * G + h % G) * max(1, -(-length // (N * G))) if length else 0
+                at = length - 1 - at if (node + h) % 2 else at     # from both ends
+                key = c.kn[s, node, h // G] if at < 0 or at >= length or (node + 3 * h) % 11 == 0 else c.pre[s][0][at, h // G]
+                c.q[s, node, h] = (4 * key.float()).to(dtype)
+    if dtype == torch.float32:
+        c.check(c.run(split_tokens=split))
+    else:
+        check(c, c.run(split_tokens=split))

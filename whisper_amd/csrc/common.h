@@ -215,7 +215,8 @@ int launch_attn_decode(const AttnArgs& a, hipStream_t st);     // n_q == 1, wave
 int launch_attn_combine(const AttnArgs& a, hipStream_t st);    // the combine a deferred launch_attn_decode left out
 int launch_kv_append(const AttnArgs& a, hipStream_t st);       // prompt pass: write the k/v rows of a.B rows into the paged cache
 int launch_attn_rows(const AttnArgs& a, hipStream_t st);       // many queries, non-causal, dense K/V (fp32 encoder path)
-int launch_attn_flash_bf16(const AttnArgs& a, hipStream_t st); // MFMA flash attention, dense bf16 K/V, non-causal
+// MFMA flash attention, dense bf16 K/V, non-causal; fine: probabilities in two bf16 numbers each (split_probs)
+int launch_attn_flash_bf16(const AttnArgs& a, hipStream_t st, bool fine = false);
 
 // ---- decoder cross-attention on the encoder output (xattn.hip) ---------------------------------------------
 struct XQTildeArgs {                     // q~[row][h][:] = s * Wk_h^T bf16((bias + sum of split-K tiles) * s)
@@ -295,6 +296,22 @@ struct BeamArgs {
     int without_timestamps = 1, suppress_blank = 1, max_initial_ts = 50;
 };
 int launch_beam_step(const BeamArgs& s, hipStream_t st);   // topk -> select -> gather -> commit (position += 1)
+
+// Eight probabilities as the sum of two bf16 numbers each, for two products with the same values.  The first is rounded from a value 2^-7 lower, so that
+// the second, what is left, is above 0 where p is (an infinite value times 0 is NaN) and at most 2^-7 + 2^-8 of p: off by half a step of that,
+// 2^-14.4 p, where one bf16 number is off by 2^-8, as much as the rounding of the result.
+// What the second product costs and gives, tree attention, us with two numbers / with one (distance from 64 bits over the result's: 0.0017 with two, of
+// which all is the rounding of the result; 0.0022 to 0.0025 with one): 16 x 24 rows, 20 heads of 64, 30-420 tokens 17.2 / 15.7; 64 single tokens
+// 31.7 / 30.6; 16 x 24 rows, 4000-16000 tokens 183 / 182; where the matrix pipe is the bound, 8 x 64 nodes, 32 heads on 8 of 128, 40000-131072
+// tokens 1012 / 758, 16 x 32 rows, 8 heads of 128, 8000-16384 tokens 198 / 176.  A drafted pass and the decoder's single steps (28 rows, 2
+// windows): 0.0063 of the largest logit apart with two in both attentions, 0.022 with one in both, 0.036 with one in the cross-attention.
+__device__ __forceinline__ void split_probs(f32x4 a, f32x4 b, bf16x8& hi, bf16x8& lo) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        hi[j] = (bf16)(a[j] * 0.9921875f); lo[j] = (bf16)(a[j] - (float)hi[j]);
+        hi[4 + j] = (bf16)(b[j] * 0.9921875f); lo[4 + j] = (bf16)(b[j] - (float)hi[4 + j]);
+    }
+}
 
 // ---- paged cache (pages.hip) and tree attention / verification (tree.hip) ----------------------------------
 // Every call runs with its buffers' device current and restores the caller's on the way out.

@@ -1606,7 +1606,7 @@ int wx_draft_logits(wx_engine* e, const wx_cache* c, const wx_draft_pass* p, voi
                 }
             } else {
                 a.q_sb = a.o_sb = (int64_t)per_window * d; a.q_sq = a.o_sq = d; a.n_q = per_window; a.B = windows;
-                WX_TRY(dtp == DT_BF16 ? launch_attn_flash_bf16(a, st) : launch_attn_rows(a, st));
+                WX_TRY(dtp == DT_BF16 ? launch_attn_flash_bf16(a, st, true) : launch_attn_rows(a, st));
             }
         }
         WX_TRY(residual(w.att, d, L.xo, L.xo_pk, L.xbo, s_dd, L.ln2_g, L.ln2_b));

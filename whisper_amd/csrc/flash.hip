@@ -27,7 +27,10 @@ constexpr float FA_LOG2E = 1.4426950408889634f;
 // launch_bounds(256, 3): three waves per SIMD (158 VGPRs, no spills).  The softmax is VALU work (~200 instructions per lane
 // per 64-key tile) that can only overlap the MFMAs of ANOTHER wave: at the compiler's default allocation (204 registers, two
 // waves per SIMD) a launch took 1439 us, at three 1082 us; four needs 128 registers, spills, and takes 3518 us.
-__global__ __launch_bounds__(256, 3) void attn_flash_bf16_kernel(AttnArgs a) {
+// FINE: the probabilities keep 15 bits for the product with the values, as the decode path's attention keeps 32: the cross-attention of drafted passes,
+// whose ids are to be the decode path's (two waves a SIMD: its registers).
+template <bool FINE>
+__global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) char lds[2 * (FA_KBYTES + FA_VBYTES)];
     // 1-D grid, XCD-aware: blocks that share an XCD (blockIdx % 8) take ALL query blocks of one (batch, head) before the
     // next, so a head's K/V (384 KB) is fetched into one L2 instead of all eight (measured: 4.2 GB -> of L2 misses per launch).
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(256, 3) void attn_flash_bf16_kernel(AttnArgs a) {
                 }
         }
         // ---- online softmax, query on the lane -------------------------------------------------------------
-        bf16x8 pf[2][2];
+        bf16x8 pf[2][2], pl[2][2];
 #pragma unroll
         for (int qt = 0; qt < 2; ++qt) {
             float mt = acc_s[0][qt][0];
@@ -150,9 +153,17 @@ __global__ __launch_bounds__(256, 3) void attn_flash_bf16_kernel(AttnArgs a) {
             }
             // k-slot order of the P^T operand = key order of the S^T accumulators: step s takes tiles 2s and 2s+1
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < 2; ++s) {
+                if constexpr (FINE) {
+                    f32x4 p0, p1;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { pf[qt][s][j] = (bf16)p[2 * s][j]; pf[qt][s][4 + j] = (bf16)p[2 * s + 1][j]; }
+                    for (int j = 0; j < 4; ++j) { p0[j] = p[2 * s][j]; p1[j] = p[2 * s + 1][j]; }
+                    split_probs(p0, p1, pf[qt][s], pl[qt][s]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { pf[qt][s][j] = (bf16)p[2 * s][j]; pf[qt][s][4 + j] = (bf16)p[2 * s + 1][j]; }
+                }
+            }
         }
         // ---- O^T += V^T P^T ------------------------------------------------------------------------------------
         const int tq = r >> 2, tp = r & 3;
@@ -168,7 +179,10 @@ __global__ __launch_bounds__(256, 3) void attn_flash_bf16_kernel(AttnArgs a) {
                 const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 const bf16x8 vf = __builtin_bit_cast(bf16x8, both);
 #pragma unroll
-                for (int qt = 0; qt < 2; ++qt) acc_o[dt][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qt][s], acc_o[dt][qt], 0, 0, 0);
+                for (int qt = 0; qt < 2; ++qt) {
+                    acc_o[dt][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qt][s], acc_o[dt][qt], 0, 0, 0);
+                    if constexpr (FINE) acc_o[dt][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[qt][s], acc_o[dt][qt], 0, 0, 0);
+                }
             }
         }
         if (more) store_tile((t + 1) & 1);
@@ -195,11 +209,12 @@ __global__ __launch_bounds__(256, 3) void attn_flash_bf16_kernel(AttnArgs a) {
     }
 }
 
-int launch_attn_flash_bf16(const AttnArgs& a, hipStream_t st) {
+int launch_attn_flash_bf16(const AttnArgs& a, hipStream_t st, bool fine) {
     if (a.dt != DT_BF16 || !a.Q || !a.K || !a.V || !a.O || a.n_q <= 0 || a.n_keys <= 0 || a.B <= 0 || a.H <= 0) return -1;
     if ((a.q_sb | a.q_sq | a.q_sh | a.kv_sbh) % 8 != 0 || (a.o_sb | a.o_sq | a.o_sh) % 4 != 0) return -1;
     dim3 grid((unsigned)(((a.n_q + 127) / 128) * ((a.B * a.H + 7) / 8 * 8)));
-    hipLaunchKernelGGL(attn_flash_bf16_kernel, grid, dim3(256), 0, st, a);
+    if (fine) hipLaunchKernelGGL(attn_flash_bf16_kernel<true>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(attn_flash_bf16_kernel<false>, grid, dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 

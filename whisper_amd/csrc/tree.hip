@@ -308,11 +308,9 @@ template <int D, int RT> struct RowState {
     template <int NS, int VROW> __device__ __forceinline__ void add(const f32x4 (&p)[NS][RT], const char* vb, int g, int r, bf16) {
 #pragma unroll
         for (int h = 0; h < NS / 2; ++h) {
-            bf16x8 pf[RT];
+            bf16x8 pf[RT], pl[RT];
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { pf[t][j] = (bf16)p[2 * h][t][j]; pf[t][4 + j] = (bf16)p[2 * h + 1][t][j]; }
+            for (int t = 0; t < RT; ++t) split_probs(p[2 * h][t], p[2 * h + 1][t], pf[t], pl[t]);
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
                 // lane (g, r) receives V[32 h + 16 u + 4 g + j][16 d + r], j = 0..3, for u = 0, 1
@@ -321,8 +319,12 @@ template <int D, int RT> struct RowState {
                 const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 16 * VROW));
                 const bf16x8 vf = __builtin_bit_cast(bf16x8, (i16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                for (int t = 0; t < RT; ++t) o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], o[d][t], 0, 0, 0);
+                for (int t = 0; t < RT; ++t) {
+                    o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], o[d][t], 0, 0, 0);
+                    o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[t], o[d][t], 0, 0, 0);
+                }
             }
+            if (RT > 1) __builtin_amdgcn_sched_barrier(0);                         // the other half is split when this one is done with: registers
         }
     }
     template <int NS, int VROW> __device__ __forceinline__ void add(const f32x4 (&p)[NS][RT], const char* vb, int g, int r, float) {
@@ -845,15 +847,13 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto pack = [&](const f32x4 (&s)[NS][RT], Frag (&pf)[RT][2]) {
+        auto pack = [&](const f32x4 (&s)[NS][RT], Frag (&pf)[RT][2], Frag (&pl)[RT][2]) {
 #pragma unroll
             for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) { pf[t][h][x] = (T)s[2 * h][t][x]; pf[t][h][4 + x] = (T)s[2 * h + 1][t][x]; }
+                for (int h = 0; h < 2; ++h) split_probs(s[2 * h][t], s[2 * h + 1][t], pf[t][h], pl[t][h]);
         };
-        auto add = [&](const char* vb, const Frag (&pf)[RT][2]) {
+        auto add = [&](const char* vb, const Frag (&pf)[RT][2], const Frag (&pl)[RT][2]) {
             constexpr int AHEAD = 2;
             Frag vf[AHEAD + 1][2];
             auto read = [&](int d) {
@@ -875,10 +875,14 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int t = 0; t < RT; ++t) st.o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d % (AHEAD + 1)][h], pf[t][h], st.o[d][t], 0, 0, 0);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) st.o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d % (AHEAD + 1)][h], pl[t][h], st.o[d][t], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        Frag pf[RT][2];
+        Frag pf[RT][2], pl[RT][2];
         const int count = __builtin_amdgcn_readfirstlane(j.count);
         if (n_tiles > 0) {
             __builtin_amdgcn_s_waitcnt(0);                                          // the counts below are of tiles' loads only (the builtin, so
@@ -903,7 +907,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
             };
             if (row0 < count * G) {
                 for (int t = 0; t < n_tiles; ++t) {
-                    if (t > 0) add(lds + ((t - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
+                    if (t > 0) add(lds + ((t - 1) & (RING - 1)) * 2 * HALF + HALF, pf, pl);
                     f32x4 s[NS][RT];
                     scores(lds + (t & (RING - 1)) * 2 * HALF, s);
                     if (late && t + 1 < n_tiles) landed(t + 1);
@@ -921,11 +925,11 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
                                     for (int q = 0; q < RT; ++q) s[k][q][x] = -INFINITY;
                     }
                     st.template softmax<NS>(s, cc);
-                    pack(s, pf);
+                    pack(s, pf, pl);
                     if (!late && t + 1 < n_tiles) landed(t + 1);
                     barrier();
                 }
-                add(lds + ((n_tiles - 1) & (RING - 1)) * 2 * HALF + HALF, pf);
+                add(lds + ((n_tiles - 1) & (RING - 1)) * 2 * HALF + HALF, pf, pl);
             } else {                                                               // a wave of nodes that are not there only brings its rows
                 for (int t = 0; t < n_tiles; ++t) {
                     if (late && t + 1 < n_tiles) landed(t + 1);
@@ -970,8 +974,8 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
 #pragma unroll
                     for (int q = 0; q < RT; ++q) if (!((mask[q] >> (16 * k + 4 * g + x)) & 1)) s[k][q][x] = -INFINITY;
             st.template softmax<NS>(s, cc);
-            pack(s, pf);
-            add(lds + HALF, pf);
+            pack(s, pf, pl);
+            add(lds + HALF, pf, pl);
             if (any_odd) add_odd_values<T, D, RT, NS>(c, a, p, j, table, head_off, page_e, 0, s, mask, st, g, r);
         }
     }
