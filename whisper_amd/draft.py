@@ -2,10 +2,16 @@
 from, and how candidates become a tree.  ``WhisperEngine.decode_draft`` is the loop that uses them.
 
 A drafter is called with the ids of every row so far (prompt included) and the number of ids wanted, and returns for every row a list of
-candidate continuations (lists of ids; none, one or several, of any length)."""
+candidate continuations (lists of ids; none, one or several, of any length).  A row that needs none (it is finished, or at its limit) is
+given as its prompt, and what comes back for it is not looked at.  ``EngineLanes`` calls one drafter from the threads of all lanes.
+
+A drafter that needs the audio has a method ``listening(engine, mel, win_stride, row_stride, n_valid_frames, B)``: a context manager that
+``transcribe_mel`` enters with the arguments of ``engine``'s last ``encode`` and leaves when these windows are decoded."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import threading
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -113,14 +119,34 @@ class NgramDraft:
 
 
 class EngineDraft:
-    """Drafts from another engine with the same vocabulary (a smaller model) that has encoded the same windows: its greedy continuation of
-    every row."""
+    """Drafts from another engine with the same vocabulary (a smaller model): its greedy continuation of every row.  ``transcribe_mel`` has
+    it encode each batch of windows as well (``listening``); where ``decode_draft`` is called directly, it must have encoded the same windows.
+    The helper serves one batch at a time: lanes that share it decode in turn."""
 
     def __init__(self, engine):
         self.engine = engine
+        self._turn = vars(engine).setdefault("_draft_turn", threading.RLock())     # one for each helper, whatever EngineDraft it is in
+
+    @contextlib.contextmanager
+    def listening(self, engine, mel, win_stride: int, row_stride: int, n_valid_frames: int, B: int):
+        helper = self.engine
+        if helper is engine:
+            raise ValueError("an engine cannot draft for itself: a replica() can")
+        if (helper.dims.n_vocab, helper.dims.n_mels, helper.torch_device) != (engine.dims.n_vocab, engine.dims.n_mels, engine.torch_device):
+            raise ValueError("the drafting engine needs the same vocabulary, number of mel bands and device")
+        if helper.max_batch < B:
+            raise ValueError(f"the drafting engine takes {helper.max_batch} windows a batch, {B} are needed")
+        with self._turn:
+            helper.encode(mel, win_stride, row_stride, n_valid_frames, B)
+            try:
+                yield self
+            finally:
+                if helper.torch_device.type == "cuda":                              # the next batch may be on another stream
+                    torch.cuda.current_stream(helper.torch_device).synchronize()
 
     def __call__(self, rows: Sequence[Sequence[int]], k: int) -> List[List[List[int]]]:
         room = self.engine.dims.n_text_ctx - 1
         if any(len(r) > room for r in rows):
             return [[] for _ in rows]
-        return [[t] for t in self.engine.decode_rows(rows, max_new_tokens=k, suppress_blank=False)["tokens"]]
+        with self._turn:
+            return [[t] for t in self.engine.decode_rows(rows, max_new_tokens=k, suppress_blank=False)["tokens"]]

@@ -7,6 +7,7 @@ Replaces what the reference obtains from ``whisper.load_model(...)`` + ``model.t
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Dict, List, Optional, Sequence
 
@@ -523,7 +524,7 @@ class WhisperEngine:
                        prompt: Sequence[int], beam_size: Optional[int] = None, patience: float = 1.0, draft=None, **decode_kw) -> Dict[str, object]:
         """Decode windows [window_lo, window_hi) of a whole-file mel ``[n_mels, ld]`` in batches of ``max_batch`` windows
         (greedy) or ``max_batch // beam_size`` windows (beam search: rows = windows x beams).  ``draft``: greedy by ``decode_draft`` with
-        this drafter ("ngram": ``NgramDraft()``)."""
+        this drafter ("ngram": ``NgramDraft()``; an ``EngineDraft``'s engine encodes every batch as well)."""
         if draft is not None and beam_size:
             raise ValueError("draft and beam_size exclude each other")
         if isinstance(draft, str):
@@ -547,7 +548,9 @@ class WhisperEngine:
                 r = self.decode_beam(B, prompt, beam_size=int(beam_size), patience=patience, **decode_kw)
                 toks += r["tokens"]; sums += r["sum_logprobs"]; nsp += r["no_speech_probs"]
             elif draft is not None:
-                r = self.decode_draft([list(prompt)] * B, draft, **decode_kw)
+                listening = getattr(draft, "listening", None)
+                with contextlib.nullcontext() if listening is None else listening(self, view, N_FRAMES, ld, n_content_frames - w0 * N_FRAMES, B):
+                    r = self.decode_draft([list(prompt)] * B, draft, **decode_kw)
                 toks += r["tokens"]; sums += r["sum_logprobs"]; nsp += r["no_speech_probs"]
             else:
                 r = self.decode_greedy(B, prompt, **decode_kw)

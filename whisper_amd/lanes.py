@@ -217,6 +217,8 @@ class EngineLanes:
         per = e0.max_batch if not beam_size else max(1, e0.max_batch // int(beam_size))
         if e0.torch_device.type == "cuda":
             torch.cuda.current_stream(e0.torch_device).synchronize()  # the mel was produced on the caller's stream
+        if any(getattr(decode_kw.get("draft"), "engine", None) is e for e in self.engines):
+            raise ValueError("a lane's engine cannot draft for the lanes: a replica() can")
         spans = [(w0, min(w0 + per, window_hi)) for w0 in range(window_lo, window_hi, per)]
 
         def one(engine, span):
