@@ -442,12 +442,14 @@ class WhisperEngine:
         begin = True
         while any(live):
             trees = [([tok.eot], [-1])] * n
-            # the first id after the prompt has a mask of its own: one node
-            asked = [[] for _ in range(n)] if begin or n_nodes == 1 else drafter(rows, n_draft)
+            # ids below the root that still count; the first id after the prompt has a mask of its own: one node
+            deep = [min(limit - (len(rows[b]) - n_prompt[b]) - 1, ctx - len(rows[b])) if live[b] and not begin and n_nodes > 1 else 0 for b in range(n)]
+            asked: Sequence[Sequence[Sequence[int]]] = [[]] * n
+            if any(d > 0 for d in deep):
+                asked = drafter([list(r) if d > 0 else r[:p] for r, d, p in zip(rows, deep, n_prompt)], n_draft)
             for b in range(n):
                 if live[b]:
-                    deep = min(limit - (len(rows[b]) - n_prompt[b]) - 1, ctx - len(rows[b]))      # ids below the root that still count
-                    trees[b] = draft_tree(rows[b][-1], [] if begin else asked[b], n_nodes, max(0, deep), tok.eot)
+                    trees[b] = draft_tree(rows[b][-1], asked[b] if deep[b] > 0 else [], n_nodes, max(0, deep[b]), tok.eot)
             width = max(len(t) for t, _ in trees)
             ids, par = np.full((n, width), tok.eot, np.int32), np.full((n, width), -1, np.int32)
             for b, (t, u) in enumerate(trees):
