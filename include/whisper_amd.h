@@ -293,8 +293,9 @@ int wx_cache_compact(const wx_cache* c, int32_t* d_n_live, void* stream);
  * committed tokens directly (NULL: a chain).  d_counts[i] (NULL: n_nodes) nodes are there; the rows of the others, and of a sequence
  * id -1 (padding of a batch), come out as 0.  With d_kn / d_vn the nodes' keys and values are appended behind the committed tokens by the same
  * call (as wx_cache_append does; the ids must be distinct then), without (both NULL) they lie there.  A sequence id out of range, rows that are not reserved or
- * whose pages another slot holds too, and a second entry of the same id in an appending call give rows of NaN and append nothing.  The
- * rows of a sequence with a page number outside the pool, and of a node with a parent out of range and its descendants, are NaN as well.  n_nodes == 1 is the ordinary decode step.  n_head: query heads, a multiple of n_kv_head up to 16 x as many; head h reads key/value head
+ * whose pages another slot holds too, and a second entry of the same id in an appending call give rows of NaN and append nothing; so do,
+ * but for the appending, sequences with a page number outside the pool.  All rows of such an entry are NaN, those of nodes that are not there as
+ * well; of an entry of no nodes only the id and the lengths are looked at.  The rows of a node with a parent out of range and of its descendants are NaN.  n_nodes == 1 is the ordinary decode step.  n_head: query heads, a multiple of n_kv_head up to 16 x as many; head h reads key/value head
  * h / (n_head / n_kv_head).  Strides in elements: heads' rows are contiguous and 16-byte aligned.  Softmax and sums in fp32; on bf16
  * caches the probabilities enter the product with the values as two bf16 numbers each (16 bits).  What masked rows hold (NaN, infinities) has no effect.
  * split_tokens: the committed tokens are cut into pieces that workgroups take side by side; 0 = by the size of the batch; > 0 = pieces

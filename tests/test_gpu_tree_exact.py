@@ -84,3 +84,59 @@ def test_no_key_is_lost(dtype, lens, N, heads, kv_heads, D, PS, split):
         c.check(c.run(split_tokens=split))
     else:
         check(c, c.run(split_tokens=split))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("lens,N,heads,kv_heads,D,PS", FORMS + [([1500, 700, 900], 24, 3, 3, 64, 16), ([3000, 1100], 6, 4, 2, 128, 16)])
+@pytest.mark.parametrize("split", [0, 128])
+def test_every_row_of_a_refused_entry_is_nan(dtype, lens, N, heads, kv_heads, D, PS, split):
+    """in whole sequences and in pieces, nodes that are not there included; all other entries stay as they are"""
+    n = len(lens)
+    c = Case(lens, N, heads, kv_heads, D, PS, dtype, seed=5, counts=[max(1, N - 2)] * n)
+    c.append = False
+    kn, vn = c.kn.cuda(), c.vn.cuda()
+    run = lambda slots, **kw: c.cache.attend(c.layer, i32(slots), c.q.cuda(), parents=i32(c.par), counts=i32(c.counts), split_tokens=split, **kw)  # noqa: E731
+    c.cache.append(i32(c.slots), c.kn.cuda(), c.vn.cuda(), counts=i32(c.counts), layer=c.layer)
+    good = run(c.slots)
+    assert torch.isfinite(good).all() and not good[:, max(1, N - 2):].any()
+
+    def alike(out, rest, slots):
+        if split or np.array_equal(slots, c.slots):
+            assert torch.equal(out[rest], good[rest])
+        else:                                                      # another batch is cut elsewhere: each side's rounding (bf16: half a step each) and its sums in 32 bits
+            torch.testing.assert_close(out[rest], good[rest], rtol=2.0 ** -7 if dtype == BF16 else 0, atol=1e-3)
+
+    def refused(at, slots=c.slots, **kw):
+        out = run(slots, **kw)
+        assert torch.isnan(out[at]).all(), (at, int(torch.isnan(out[at]).sum()), out[at].numel())
+        alike(out, [i for i in range(n) if i != at], slots)
+    table, held, refs = c.cache.table, c.cache.held, c.cache.refs
+    for at in (0, n - 1):
+        s = int(c.slots[at])
+        other = c.slots.copy()
+        for bad in (n + 1, -2, 10 ** 6):
+            other[at] = bad
+            refused(at, other)
+        was = int(held[s])
+        held[s] = max(0, -(-(int(c.lens[at]) + max(1, N - 2)) // PS) - 1)
+        refused(at)
+        held[s] = was
+        for page in (0, int(c.lens[at]) // PS):                    # the first piece's, the last's
+            was = int(table[s, page])
+            for bad in (-1, 10 ** 8):
+                table[s, page] = bad
+                refused(at)
+            table[s, page] = was
+        page = int(table[s, int(c.lens[at]) // PS])
+        refs[page] = 2
+        refused(at, k=kn, v=vn)
+        refs[page] = 1
+    if n > 1:
+        twice = c.slots.copy()
+        twice[n - 1] = twice[0]
+        refused(n - 1, twice, k=kn, v=vn)
+    pad = c.slots.copy()
+    pad[0] = -1
+    out = run(pad)
+    assert not out[0].any()
+    alike(out, range(1, n), pad)

@@ -28,7 +28,7 @@ struct TreePlan {
     int pieces;              // ... and places for their parts
     int rows;                // rows a workgroup
     int merge_rows;          // rows a workgroup of the merge (a power of two); the rest of its threads share their pieces
-    float* part;             // [pieces][n_kv_head][row_blocks][rows][D + 2]: output, maximum and sum (sequences in more than one piece)
+    float* part;             // [pieces][n_kv_head][row_blocks][rows][D + 2]: output, maximum (NaN: refused) and sum (sequences in more than one piece)
 };
 
 __device__ __forceinline__ int tree_tiles_of(const wx_cache& c, const wx_tree_attn& a, const TreePlan& p, int i, int kt) {
@@ -672,7 +672,6 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
                 v += *reinterpret_cast<const f32x4*>(o + (w * RT * 16 + row) * OROW + x);
             }
             const int node = at / G;
-            if (j.ok == 2) L = __builtin_nanf("");
             if (whole) {
                 T* out = reinterpret_cast<T*>(a.d_out) + j.i * a.o_seq + node * a.o_node + (j.kh * G + at % G) * a.o_head + half * 64 + x;
                 if (j.ok == 0 || (j.ok == 1 && node >= j.count)) v = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -683,7 +682,7 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
                 float* to = part + (int64_t)row * (D + 2);
                 *reinterpret_cast<f32x2*>(to + half * 64 + x) = f32x2{v[0], v[1]};
                 *reinterpret_cast<f32x2*>(to + half * 64 + x + 2) = f32x2{v[2], v[3]};
-                if (x == 0 && half == 0) { to[D] = M; to[D + 1] = L; }
+                if (x == 0 && half == 0) { to[D] = j.ok == 2 ? __builtin_nanf("") : M; to[D + 1] = L; }
             }
         }
     }
@@ -1007,7 +1006,7 @@ __global__ __launch_bounds__(64 * TRW, 2) void tree_attention_rows_kernel(TreeAr
                 *reinterpret_cast<f32x2*>(to + 16 * d + 4 * g) = f32x2{st.o[d][t][0], st.o[d][t][1]};
                 *reinterpret_cast<f32x2*>(to + 16 * d + 4 * g + 2) = f32x2{st.o[d][t][2], st.o[d][t][3]};
             }
-            if (g == 0) { to[D] = st.m[t]; to[D + 1] = j.ok == 2 ? __builtin_nanf("") : l; }
+            if (g == 0) { to[D] = j.ok == 2 ? __builtin_nanf("") : st.m[t]; to[D + 1] = l; }
         }
     }
     }
@@ -1059,6 +1058,7 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
     const float* part = p.part + ((((int64_t)first * c.n_kv_head + kh) * p.row_blocks + min(row, rows - 1) / p.rows) * p.rows + min(row, rows - 1) % p.rows) * (D + 2);
     // four pieces' loads at a time, one running maximum (a launch of this size is bound by the loads' latency)
     float M = -INFINITY, L = 0.f;
+    bool refused = false;                                                           // by any piece: a maximum is never NaN otherwise
     f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int q0 = 4 * group; q0 < pieces; q0 += 4 * groups) {
         float m[4], l[4];
@@ -1071,7 +1071,7 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
         }
         float mn = M;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mn = fmaxf(mn, m[q]);
+        for (int q = 0; q < 4; ++q) { mn = fmaxf(mn, m[q]); refused |= m[q] != m[q]; }
         const float old = M == mn ? 1.f : __builtin_amdgcn_exp2f((M - mn) * cc);
         M = mn;
         L *= old; v *= old;
@@ -1085,11 +1085,12 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
     }
     if (groups > 1) {                                                               // the groups' parts, in order
         s_v[slot][tid % TPR] = v;
-        if (x == 0) { s_m[slot] = M; s_l[slot] = L; }
+        if (x == 0) { s_m[slot] = refused ? __builtin_nanf("") : M; s_l[slot] = L; }
         __syncthreads();
         if (group > 0) return;
         for (int o = slot + p.merge_rows; o < RPB; o += p.merge_rows) {
             const float mo = s_m[o], mn = fmaxf(M, mo);
+            refused |= mo != mo;
             const float fa = M == mn ? 1.f : __builtin_amdgcn_exp2f((M - mn) * cc), fb = mo == mn ? 1.f : __builtin_amdgcn_exp2f((mo - mn) * cc);
             M = mn;
             L = L * fa + s_l[o] * fb;
@@ -1099,7 +1100,7 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(wx_cache c, w
     if (row >= rows) return;
     const int node = row / G;
     T* out = reinterpret_cast<T*>(a.d_out) + i * a.o_seq + node * a.o_node + (kh * G + row % G) * a.o_head + x;
-    const int kind = seq == -1 || node >= count ? 0 : s_wrong[node] ? 2 : 1;
+    const int kind = refused ? 2 : seq == -1 || node >= count ? 0 : s_wrong[node] ? 2 : 1;
     store4<T>(out, kind == 1 ? v * (1.f / L) : f32x4{1.f, 1.f, 1.f, 1.f} * (kind == 0 ? 0.f : __builtin_nanf("")));
 }
 
