@@ -300,7 +300,7 @@ int wx_cache_compact(const wx_cache* c, int32_t* d_n_live, void* stream);
  * caches the probabilities enter the product with the values as two bf16 numbers each (16 bits).  What masked rows hold (NaN, infinities) has no effect.
  * split_tokens: the committed tokens are cut into pieces that workgroups take side by side; 0 = by the size of the batch; > 0 = pieces
  * of that many tokens (rounded up to a tile of 16 to 64 tokens, and to a 256th of what a table holds), so that a sequence's result does
- * not depend on what else is in the batch.  d_out may be d_q. */
+ * not depend on what else is in the batch, nor on how wide the batch is padded (n_nodes).  d_out may be d_q. */
 typedef struct {
     int32_t layer, n, n_nodes, n_head;
     const int32_t *d_seqs, *d_parents, *d_counts;

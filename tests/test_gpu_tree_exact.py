@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import kv_model as km
-from test_gpu_tree import BF16, Case, i32
+from test_gpu_tree import BF16, Case, i32, trees
+from whisper_amd.kvcache import PagedKVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +141,30 @@ def test_every_row_of_a_refused_entry_is_nan(dtype, lens, N, heads, kv_heads, D,
     out = run(pad)
     assert not out[0].any()
     alike(out, range(1, n), pad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("G,kv_heads,D", [(1, 2, 64), (3, 2, 64), (8, 1, 64), (16, 1, 64), (1, 2, 128), (2, 4, 128), (4, 2, 128), (16, 1, 128)])
+@pytest.mark.parametrize("longest,split", [(100, 64), (3000, 64), (3000, 300), (3000, 1 << 20), (20000, 64)])
+def test_a_fixed_cut_does_not_see_the_width_of_the_batch(dtype, G, kv_heads, D, longest, split):
+    """a sequence of three nodes, alone and among sequences that pad the batch to more nodes: the same bits"""
+    n, W, PS = 3, 64, 64
+    H, g = G * kv_heads, torch.Generator().manual_seed(G)
+    lens = [longest, longest // 3, 7]
+    pages = [-(-(x + W) // PS) for x in lens]
+    c = PagedKVCache.allocate(1, kv_heads, D, sum(pages), n, max(pages), page_size=PS, dtype=dtype)
+    c.k.copy_(torch.randn(c.k.shape, generator=g).to(dtype)); c.v.copy_(torch.randn(c.v.shape, generator=g).to(dtype))
+    c.lens.copy_(i32([0] * n))
+    assert not c.reserve(i32(range(n)), i32([x + W for x in lens])).any()
+    c.lens.copy_(i32(lens))
+    q = torch.randn(n, W, H, D, generator=g).to(dtype).cuda()
+    par = i32(trees(np.random.RandomState(1), n, W))
+    want = None
+    for width in (3, 4, 5, 8, 9, 16, 17, 32, 33, 43, 64):
+        counts = i32([3, width, max(1, width - 2)])
+        out = c.attend(0, i32([0, 1, 2]), q[:, :width].contiguous(), parents=par[:, :width].contiguous(), counts=counts, split_tokens=split)[0, :3]
+        want = out if want is None else want
+        assert torch.equal(out, want), (width, float((out - want).abs().max()))
+    for width in (3, 17, 64):
+        alone = c.attend(0, i32([0]), q[:1, :width].contiguous(), parents=par[:1, :width].contiguous(), counts=i32([3]), split_tokens=split)[0, :3]
+        assert torch.equal(alone, want)

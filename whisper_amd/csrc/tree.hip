@@ -1121,13 +1121,14 @@ static hipError_t launch_rows(dim3 grid, int lds, hipStream_t st, const wx_cache
 // Which kernel, and how the work is cut.
 struct TreeForm { bool rows_form; int rt, rows, kt; };
 static TreeForm tree_form(const wx_cache& c, const wx_tree_attn& a) {
-    const int rows = a.n_nodes * (a.n_head / c.n_kv_head), es = c.precision == WX_PREC_F32 ? 4 : 2;
+    const int G = a.n_head / c.n_kv_head, rows = a.n_nodes * G, es = c.precision == WX_PREC_F32 ? 4 : 2;
     TreeForm f;
-    // Both forms measured at contexts of 4000-16000 tokens and below 500.  Heads of 128: up to 16 rows the waves share the keys (14.7 us
-    // against 20.4 at 32 x 4 rows and short contexts; 164 against 150 at long ones), above that they share the rows (16 x 32 rows: 153 us
-    // against 171; 16 x 64 rows: 169 against 225).  Heads of 64, whose tiles are half as large for the same barriers: 16 x 64 rows 249 us with
-    // the keys shared, 487 with the rows.
-    f.rows_form = c.precision == WX_PREC_BF16 && rows > (c.head_dim == 128 ? 16 : 128);
+    // us with the keys shared / the rows shared, 16 sequences, 8 key / value heads.  Heads of 128, 30-420 tokens: 20 rows 17 / 24, 32 38 / 32, 64 59 /
+    // 35; 4000-16000 tokens: 32 rows 155 / 163, 64 239 / 174, 256 764 / 315.  Heads of 64, whose tiles are half as large for the same barriers:
+    // 4000-16000 tokens: 64 rows 98 / 193, 128 144 / 202, 192 199 / 208, 256 248 / 214; 30-420: 64 39 / 33, 128 51 / 37, 256 57 / 42.
+    // With split_tokens the number of nodes must not matter (it is the widest sequence's): by the heads alone.  Heads of 128, 4 query heads: 1 node
+    // 132 / 167, 8 171 / 213, 16 270 / 233, 64 973 / 441; 2: 1 133 / 165, 16 171 / 213, 32 272 / 233.
+    f.rows_form = c.precision == WX_PREC_BF16 && (a.split_tokens > 0 ? c.head_dim == 128 && G >= 4 : rows > (c.head_dim == 128 ? 16 : 128));
     // 32 rows a wave (two row tiles for every fragment read) where they are there and the registers allow it
     f.rt = f.rows_form ? rows > 128 ? 2 : 1 : rows > 16 && c.head_dim == 64 ? 2 : 1;
     f.rows = f.rows_form ? 128 * f.rt : 16 * f.rt;
@@ -1157,19 +1158,20 @@ static TreePlan tree_plan(const wx_cache& c, const wx_tree_attn& a, const TreeFo
     int64_t takers = slots / units;
     if (5 * takers * units < 4 * slots) takers = 4 * slots / units;
     p.takers = (int)(takers > 1 ? takers : 1);
-    if (a.split_tokens > 0) {                                                       // at most 256 pieces a sequence
+    if (a.split_tokens > 0) {                                                       // at most 256 pieces a sequence, whatever n_nodes is
+        const int64_t widest = most - p.tree_tiles + (TR_NODES + f.kt - 1) / f.kt;
         p.per = (int)(((int64_t)a.split_tokens + f.kt - 1) / f.kt);
-        if (p.per < (most + 255) / 256) p.per = (int)((most + 255) / 256);
+        if (p.per < (widest + 255) / 256) p.per = (int)((widest + 255) / 256);
     }
     p.single = most <= (p.per ? p.per : 512 / f.kt + p.tree_tiles);
     p.slots = p.single ? a.n : p.per ? (int)(a.n * ((most + p.per - 1) / p.per)) : p.takers;
     p.pieces = p.single ? 0 : p.per ? p.slots : p.takers + a.n;
     // the merge: as few rows a workgroup (as many threads on a row's pieces) as leave it at most 2048 workgroups (6 sequences of up to 38255
     // tokens, 2 heads of 64, f32, shares of 128: 55 us so, 67 with every row's pieces on one group of threads); the order of the sum follows from
-    // it, so with `per` it is taken for 8 sequences whatever their number
-    const int64_t merges = units * (p.per ? 8 : a.n);
+    // it, so with `per` it is taken for 8 sequences of 8 nodes whatever their number
+    const int64_t merges = (int64_t)c.n_kv_head * (p.per ? 8 : a.n), merged = p.per ? 8 * (a.n_head / c.n_kv_head) : rows;
     p.merge_rows = 1024 / c.head_dim;
-    while (p.merge_rows > 1 && merges * ((rows + p.merge_rows / 2 - 1) / (p.merge_rows / 2)) <= 2048 * (int64_t)p.row_blocks) p.merge_rows /= 2;
+    while (p.merge_rows > 1 && merges * ((merged + p.merge_rows / 2 - 1) / (p.merge_rows / 2)) <= 2048) p.merge_rows /= 2;
     return p;
 }
 // Whether a wave alone takes a whole sequence (a key / value head, a block of rows): jobs enough to fill the chip without cutting them, and
