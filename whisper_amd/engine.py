@@ -387,8 +387,9 @@ class WhisperEngine:
                      without_timestamps: bool = True, suppress_blank: bool = True) -> Dict[str, object]:
         """Greedy decode with one prompt per window of the last encode, several ids a pass: ``drafter`` (whisper_amd/draft.py; default
         ``NgramDraft()``) proposes continuations, one decoder pass answers all of their ids over a paged cache, and the ids that agree with
-        the arg-max are kept.  The ids are greedy's own whatever the drafts (in bf16 up to the rounding of another summation order, as
-        between batch sizes); only the number of passes changes.  ``n_nodes``: most drafted ids of a row in one pass, the certain one
+        the arg-max are kept.  The ids are greedy's own whatever the drafts; only the number of passes changes.  In bf16 that holds up to
+        near-ties: a pass sums in another order, as another batch size does, and on engines that attend the encoder output (``cross_form``) it
+        attends cached keys and values, which are rounded elsewhere.  ``n_nodes``: most drafted ids of a row in one pass, the certain one
         included; ``n_draft``: longest continuation asked for.  Timestamp rules depend on the whole row: not offered here.
 
         Returns ``decode_rows``'s fields, and ``passes`` and ``accepted`` (drafted ids kept)."""
