@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import operator
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -372,12 +373,15 @@ class WhisperEngine:
         for t, what, shape in ((seqs, "seqs", (n,)), (tokens, "tokens", (n, nodes)), (parents, "parents", (n, nodes)), (counts, "counts", (n,))):
             if t is not None and (t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous()):
                 raise ValueError(f"{what} must be a contiguous int32 tensor {list(shape)} on {dev}")
+        group = operator.index(group)
+        if not 1 <= group < 1 << 31:                                  # ctypes would cut a number to 32 bits without a word
+            raise ValueError("group must be at least 1 (and a number of 32 bits)")
         stride = int(self.lib.wx_logit_stride(self.handle))
         logits = torch.empty((n, nodes, stride), dtype=torch.float32, device=dev) if want_logits else None
         need = int(self.lib.wx_draft_work_bytes(self.handle, n, nodes))
         _lib.check(min(need, 0), "wx_draft_work_bytes")
         work = torch.empty(need, dtype=torch.uint8, device=dev)
-        p = _lib.WxDraftPass(n=n, n_nodes=nodes, group=int(group), want_logits=int(want_logits), d_seqs=seqs.data_ptr(), d_tokens=tokens.data_ptr(),
+        p = _lib.WxDraftPass(n=n, n_nodes=nodes, group=group, want_logits=int(want_logits), d_seqs=seqs.data_ptr(), d_tokens=tokens.data_ptr(),
                              d_parents=None if parents is None else parents.data_ptr(), d_counts=None if counts is None else counts.data_ptr(),
                              d_logits=None if logits is None else logits.data_ptr(), d_work=work.data_ptr(), work_bytes=need)
         _lib.check(self.lib.wx_draft_logits(self.handle, cache._ref, ctypes.byref(p), self._stream()), "wx_draft_logits")
