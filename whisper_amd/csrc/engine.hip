@@ -1591,9 +1591,10 @@ int wx_draft_logits(wx_engine* e, const wx_cache* c, const wx_draft_pass* p, voi
             a.dt = dtp; a.Q = w.q; a.O = w.att; a.H = e->Ht; a.q_sh = a.o_sh = HEAD_DIM;
             a.K = (char*)e->crossK + cross_layer * i * es; a.V = (char*)e->crossV + cross_layer * i * es; a.kv_sbh = (int64_t)T * HEAD_DIM; a.n_keys = T;
             // Few rows share a window's stream in the single-token kernel (vector pipe, cut along the keys), eight at a time; more take the encoder's
-            // kernel (matrix pipe, one workgroup a window and head: one window's 1500 keys last 35 us whatever the rows).  A pass of large-v3:
-            // 1 x 8 nodes 2.2 against 3.3 ms, 4 x 8 the same, 8 x 8 4.3 against 3.5; 32 x 2 3.7 against 4.2.
-            if (few && (per_window <= 2 || (R <= 16 && (per_window <= 8 || windows == 1)))) {
+            // kernel in its fine form (matrix pipe, one workgroup a window and head: its latency over one window's 1500 keys whatever the rows).  A
+            // captured pass of large-v3, ms, single-token kernel / encoder's: 1 x 8 nodes 2.12 / 2.61, 1 x 12 2.59 / 2.64, 1 x 16 2.87 / 2.67; 2 x 8 2.21 /
+            // 2.89; 4 x 8 2.87 / 3.06; 8 x 4 2.59 / 3.05, 8 x 6 4.14 / 3.22; 16 x 4 3.26 / 3.54, 16 x 6 6.46 / 4.95.
+            if (few && (windows == 1 ? R <= 12 : per_window <= 4 || (per_window <= 8 && R <= 32))) {
                 a.q_sb = a.o_sb = d; a.n_q = 1; a.partial = w.parts;
                 a.n_split = 1;
                 while (a.n_split < DRAFT_CROSS_SPLIT && k.max_batch * e->Ht * a.n_split < 512) ++a.n_split;

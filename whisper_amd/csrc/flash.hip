@@ -28,13 +28,14 @@ constexpr float FA_LOG2E = 1.4426950408889634f;
 // per 64-key tile) that can only overlap the MFMAs of ANOTHER wave: at the compiler's default allocation (204 registers, two
 // waves per SIMD) a launch took 1439 us, at three 1082 us; four needs 128 registers, spills, and takes 3518 us.
 // FINE: the probabilities keep 15 bits for the product with the values, as the decode path's attention keeps 32: the cross-attention of drafted passes,
-// whose ids are to be the decode path's (two waves a SIMD: its registers).
-template <bool FINE>
-__global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(AttnArgs a) {
+// whose ids are to be the decode path's.  There a window has few rows and one workgroup of it for each head, whose latency is the launch's: 16 rows a
+// wave (QT = 1).
+template <bool FINE, int QT>
+__global__ __launch_bounds__(256, 3) void attn_flash_bf16_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) char lds[2 * (FA_KBYTES + FA_VBYTES)];
     // 1-D grid, XCD-aware: blocks that share an XCD (blockIdx % 8) take ALL query blocks of one (batch, head) before the
     // next, so a head's K/V (384 KB) is fetched into one L2 instead of all eight (measured: 4.2 GB -> of L2 misses per launch).
-    const int nqb = (a.n_q + 127) / 128, nbh = a.B * a.H;
+    const int nqb = (a.n_q + 64 * QT - 1) / (64 * QT), nbh = a.B * a.H;
     const int xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
     const int bh = (slot / nqb) * 8 + xcd, qb = slot % nqb;
     if (bh >= nbh) return;
@@ -42,15 +43,15 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int g = lane >> 4, r = lane & 15;
     const int n_q = a.n_q, n_keys = a.n_keys;
-    const int q0 = qb * 128 + wid * 32;
+    const int q0 = qb * (64 * QT) + wid * (16 * QT);
 
     const bf16* Qp = reinterpret_cast<const bf16*>(a.Q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
     const bf16* Kp = reinterpret_cast<const bf16*>(a.K) + ((int64_t)b * a.H + h) * a.kv_sbh;
     const bf16* Vp = reinterpret_cast<const bf16*>(a.V) + ((int64_t)b * a.H + h) * a.kv_sbh;
 
-    bf16x8 qf[2][2];
+    bf16x8 qf[QT][2];
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
+    for (int qt = 0; qt < QT; ++qt) {
         int iq = q0 + qt * 16 + r; if (iq > n_q - 1) iq = n_q - 1;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) qf[qt][ks] = *reinterpret_cast<const bf16x8*>(Qp + (int64_t)iq * a.q_sq + ks * 32 + g * 8);
@@ -78,12 +79,14 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
         }
     };
 
-    f32x4 acc_o[4][2];
+    f32x4 acc_o[4][QT];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-        for (int qt = 0; qt < 2; ++qt) acc_o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+        for (int qt = 0; qt < QT; ++qt) acc_o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run[QT], l_run[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) { m_run[qt] = -INFINITY; l_run[qt] = 0.f; }
 
     const int nt = (n_keys + FA_KT - 1) / FA_KT;
     load_tile(0);
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
         const char* kb = lds + (t & 1) * (FA_KBYTES + FA_VBYTES);
         const char* vb = kb + FA_KBYTES;
         // ---- S^T = K Q^T -------------------------------------------------------------------------------
-        f32x4 acc_s[4][2];
+        f32x4 acc_s[4][QT];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             const int row = kt * 16 + r;
@@ -103,7 +106,7 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) kf[ks] = *reinterpret_cast<const bf16x8*>(kb + row * FA_KROW + (((ks * 4 + g) ^ (row & 7)) << 4));
 #pragma unroll
-            for (int qt = 0; qt < 2; ++qt) {
+            for (int qt = 0; qt < QT; ++qt) {
                 f32x4 c = f32x4{0.f, 0.f, 0.f, 0.f};
                 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[0], qf[qt][0], c, 0, 0, 0);
                 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[1], qf[qt][1], c, 0, 0, 0);
@@ -117,13 +120,15 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = t * FA_KT + kt * 16 + g * 4 + j;
-                    if (key >= n_keys) { acc_s[kt][0][j] = -INFINITY; acc_s[kt][1][j] = -INFINITY; }
+                    if (key >= n_keys)
+#pragma unroll
+                        for (int qt = 0; qt < QT; ++qt) acc_s[kt][qt][j] = -INFINITY;
                 }
         }
         // ---- online softmax, query on the lane -------------------------------------------------------------
-        bf16x8 pf[2][2], pl[2][2];
+        bf16x8 pf[QT][2], pl[QT][2];
 #pragma unroll
-        for (int qt = 0; qt < 2; ++qt) {
+        for (int qt = 0; qt < QT; ++qt) {
             float mt = acc_s[0][qt][0];
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
@@ -179,7 +184,7 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
                 const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 const bf16x8 vf = __builtin_bit_cast(bf16x8, both);
 #pragma unroll
-                for (int qt = 0; qt < 2; ++qt) {
+                for (int qt = 0; qt < QT; ++qt) {
                     acc_o[dt][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qt][s], acc_o[dt][qt], 0, 0, 0);
                     if constexpr (FINE) acc_o[dt][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[qt][s], acc_o[dt][qt], 0, 0, 0);
                 }
@@ -190,7 +195,7 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
     }
     // ---- normalise and store: lane holds O[q = r][d = 16dt + 4g + 0..3] ---------------------------------------------
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
+    for (int qt = 0; qt < QT; ++qt) {
         float l = l_run[qt];
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
@@ -212,9 +217,10 @@ __global__ __launch_bounds__(256, FINE ? 2 : 3) void attn_flash_bf16_kernel(Attn
 int launch_attn_flash_bf16(const AttnArgs& a, hipStream_t st, bool fine) {
     if (a.dt != DT_BF16 || !a.Q || !a.K || !a.V || !a.O || a.n_q <= 0 || a.n_keys <= 0 || a.B <= 0 || a.H <= 0) return -1;
     if ((a.q_sb | a.q_sq | a.q_sh | a.kv_sbh) % 8 != 0 || (a.o_sb | a.o_sq | a.o_sh) % 4 != 0) return -1;
-    dim3 grid((unsigned)(((a.n_q + 127) / 128) * ((a.B * a.H + 7) / 8 * 8)));
-    if (fine) hipLaunchKernelGGL(attn_flash_bf16_kernel<true>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(attn_flash_bf16_kernel<false>, grid, dim3(256), 0, st, a);
+    const int rows = fine ? 64 : 128;
+    dim3 grid((unsigned)(((a.n_q + rows - 1) / rows) * ((a.B * a.H + 7) / 8 * 8)));
+    if (fine) hipLaunchKernelGGL((attn_flash_bf16_kernel<true, 1>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_flash_bf16_kernel<false, 2>), grid, dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
