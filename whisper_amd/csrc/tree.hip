@@ -417,8 +417,9 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* to, f32x4 v) {
 // Bound by the stream of keys and values.  A tile is 8 KiB of keys (straight into the matrix instruction's registers) and 8 KiB of
 // values (through the wave's own LDS, for the transposing read); the next tile's 16 loads a lane are issued as soon as the scores of
 // this one are taken, and no wave waits for another before the end, where the four states are merged through LDS.
-// Against one thread a key and head, without matrix instructions: 16 x 24 rows, 20 heads of 64, 30-420 tokens: 268 us -> 15 us (24 MB;
-// latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 31 us, 29 with SOLO (111 MB, 3.8 TB/s); 16 x 24 rows, 4000-16000 tokens: 182 us.
+// Kernel times on bf16, against one thread a key and head without matrix instructions: 16 x 24 rows, 20 heads of 64, 30-420 tokens: 268 us ->
+// 16.6 us (24 MB; latency: four tiles a wave at most); 64 x 1 row, 200-447 tokens: 85 -> 30 us with SOLO (111 MB, 3.7 TB/s); 16 x 24 rows,
+// 4000-16000 tokens, 20 heads of 64: 183 us (one launch and its merge).
 // With three waves a SIMD instead of two the vector registers spill, 64 x 1 row take 33 us, and the cut form of that build gave wrong results (cause not
 // established): no kernel here keeps vector registers in scratch memory.
 // SOLO (whole sequences, jobs enough to fill the chip: tree_solo): every wave has a job of its own and takes all of its tiles, so
@@ -693,12 +694,14 @@ __global__ __launch_bounds__(256, 2) void tree_attention_keys_kernel(TreeArgs) {
 // Eight waves, RT x 16 rows each (two waves on every SIMD of a CU).  Tiles of 64 keys go from HBM to LDS without registers
 // (global_load_lds) into a ring of four, three tiles before their use; a wave-instruction writes 1 KiB of rows in a line, so the swizzle
 // that the fragment reads need (16-byte chunk x of a row in slot x ^ (row mod chunks)) is applied to its lanes' source addresses.
-// The softmax of a tile takes the vector pipe about as long as its two products take the matrix pipe.  So waves 4-7 run half a tile
+// The softmax of a tile takes the vector pipe about as long as its products take the matrix pipe.  So waves 4-7 run half a tile
 // behind waves 0-3, a barrier each half: while one wave of a SIMD does PV(t - 1) and QK(t), the other does the softmax of its tile.
-// 8 x 64 nodes, 32 query heads on 8 of 128, 40000-131072 tokens (2.5 GB, 0.52 TFLOP): 742 us, 0.70 PFLOP/s and 3.4 TB/s.  Keys and values
-// through registers and all waves in step: 967 us; to LDS directly, in two phases: 835; scalar addresses, loads issued in the softmax's half
-// and waves without rows left out of the products: 742.  What is left, part by part (the others left out): the stream 486 us, the products
-// with their LDS reads 582 (435 without the LDS reads; these alone 471).  16 x 32 rows, 8000-16384 tokens, 8 heads of 128: 153 us, 5.2 TB/s.
+// 8 x 64 nodes, 32 query heads on 8 of 128, 40000-131072 tokens (2.5 GB, 0.52 TFLOP, 0.78 with the second product of split_probs): 1005 us back to
+// back (median of 15 replays; 1078 on average under the profiler), 0.78 PFLOP/s executed and 2.5 TB/s; with one product for the probabilities
+// 760.  That form, step by step: keys and values through registers and all waves in step 967 us; to LDS directly, in two phases: 835; scalar
+// addresses, loads issued in the softmax's half and waves without rows left out of the products: 760.  What is left, part by part (the others
+// left out): the stream 467 us, the products with their LDS reads 720, products and softmax without the stream 960.  Splitting the
+// probabilities with the products instead of with the softmax: 1020.  16 x 32 rows, 8000-16384 tokens, 8 heads of 128: 198 us, 4.0 TB/s.
 //
 // 16 bytes a lane from global memory (`from`, alike on the wave, + lane_off) to LDS address `to` + 16 x lane.  Written out because the
 // compiler, which knows of the builtin's LDS write, waits for ALL loads before every transposing LDS read, whatever they write; the waits

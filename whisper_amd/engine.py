@@ -396,6 +396,10 @@ class WhisperEngine:
         attends cached keys and values, which are rounded elsewhere.  ``n_nodes``: most drafted ids of a row in one pass, the certain one
         included; ``n_draft``: longest continuation asked for.  Timestamp rules depend on the whole row: not offered here.
 
+        It pays where rows are few: a pass takes every row to the width of the widest tree, finished rows too, and several rows already share
+        greedy's stream of the weights.  large-v3 in bf16, 100 ids, n-gram drafts of 8 against greedy: 88 ms against 150 for 1 window, 177 against
+        170 for 4, 426 against 226 for 16.
+
         Returns ``decode_rows``'s fields, and ``passes`` and ``accepted`` (drafted ids kept)."""
         from .draft import NgramDraft, draft_tree, verify_tree
         if not without_timestamps:
@@ -531,7 +535,7 @@ class WhisperEngine:
                        prompt: Sequence[int], beam_size: Optional[int] = None, patience: float = 1.0, draft=None, **decode_kw) -> Dict[str, object]:
         """Decode windows [window_lo, window_hi) of a whole-file mel ``[n_mels, ld]`` in batches of ``max_batch`` windows
         (greedy) or ``max_batch // beam_size`` windows (beam search: rows = windows x beams).  ``draft``: greedy by ``decode_draft`` with
-        this drafter ("ngram": ``NgramDraft()``; an ``EngineDraft``'s engine encodes every batch as well)."""
+        this drafter ("ngram": ``NgramDraft()``; an ``EngineDraft``'s engine encodes every batch as well), which pays for one window a batch."""
         if draft is not None and beam_size:
             raise ValueError("draft and beam_size exclude each other")
         if isinstance(draft, str):

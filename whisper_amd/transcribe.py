@@ -136,7 +136,7 @@ def transcribe(audio, language: Optional[str] = None, prompt: Union[None, str, S
 
     ``decode_kw``: ``beam_size`` (None = greedy, upstream's default for the reference's call), ``patience``,
     ``max_new_tokens``, ``without_timestamps``, ``draft`` (windows mode, greedy: several ids a decoder pass, "ngram" or a drafter of
-    whisper_amd/draft.py).
+    whisper_amd/draft.py; faster than plain greedy for one window, slower for several in one batch: ``WhisperEngine.decode_draft``).
 
     Returns ``{"text", "confidence", "chunks_processed"}`` plus ``language``, ``tokens`` (per window),
     ``avg_logprob`` and ``no_speech_prob`` (per window).
